@@ -327,6 +327,63 @@ TL_API int32_t tl_decode_attention(tl_ctx* ctx, const void* q, const void* k_cac
                                    int64_t head_dim, int64_t kv_len, int64_t kv_capacity, float scale,
                                    const float* mask);
 
+/* ---- a decode step over a paged cache: sequences of their own lengths, each on pages of its own ------------------------------
+ * (No counterpart in the reference, whose cache is one [batch, n_kv_heads, capacity, head_dim] tensor with one length for all
+ * sequences, packages/qwen3-browser/src/model.ts:240-312; that tensor is the case page_size == capacity, page_table[b] == {b}, so
+ * tl_paged_append serves tl_attention and tl_decode_attention too.)
+ * A sequence's position p lies in page page_table[seq * max_pages + p / page_size] at p % page_size; a page holds
+ * [n_kv_heads, page_size, head_dim] elements of dtype, k_pages and v_pages [n_pages] of them.  Entries of the table behind a
+ * sequence's last position are not read.
+ * positions[t] is the position of token t in its sequence and token_seq[t] that sequence (NULL: token t belongs to sequence t).
+ * A negative position marks a token that is not there (a padded batch): nothing of it is read or written, only tl_paged_attention
+ * writes zeros for it.  positions, token_seq and page_table are int32 on the device, read when the kernel runs, so that a captured step replays
+ * with new ones.  What only the kernel can see -- a position past max_pages * page_size or the rotation tables, a
+ * sequence or page that is not there -- skips that token (a page of the past: those keys), touches no memory, and is reported by the next
+ * tl_sync as TL_ERR_INVALID_ARG. */
+typedef struct tl_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* page_table; /* [n_seqs, max_pages] */
+  int64_t n_pages;
+  int32_t page_size; /* any, 1 among them */
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t dtype; /* TL_F32, TL_F16 or TL_BF16: of the pages and of q, k, v and the outputs */
+  int32_t n_seqs;
+  int32_t max_pages;
+} tl_paged_cache;
+/* tl_paged_append: the per-head norm of q and k (tl_rmsnorm with cols = head_dim, where the weight is given), the rotation of tl_rope at
+ * each token's position (where the tables are given, f32 [table_rows, head_dim / 2]) and the append of k and v, one launch.
+ * q [tokens, n_heads, head_dim], k and v [tokens, n_kv_heads, head_dim] with any strides in elements between tokens and between heads
+ * (the columns of one fused product, or the [heads, tokens, head_dim] order of tl_rope); q_out likewise.  q may be NULL
+ * (k and v alone) and q_out may be q itself with q's strides.  Two tokens of a call at the same position of a sequence leave
+ * that position undefined.  head_dim is even, at most 1024. */
+TL_API int32_t tl_paged_append(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t* positions, const int32_t* token_seq, int64_t tokens,
+                               const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t n_heads, void* q_out,
+                               int64_t out_token_stride, int64_t out_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                               const void* v, int64_t v_token_stride, int64_t v_head_stride, const void* q_weight, const void* k_weight,
+                               int32_t weight_dtype, float eps, const float* cos_table, const float* sin_table, int64_t table_rows);
+/* tl_paged_attention: one query token per row against its own sequence, the token's own key and value among the appended ones.
+ * q [tokens, n_heads, head_dim] with strides as above, query head h reads kv head h / (n_heads / n_kv_heads), out is [tokens, n_heads, head_dim].
+ * Token t at position p sees the keys j <= p, with window > 0 only those with p - j < window:
+ *   x_j = q . k_j * scale;  softcap > 0: x_j = softcap * tanh(x_j / softcap);  slopes: x_j += slopes[h] * (j - p)  (f32 [n_heads])
+ *   out = sum_j softmax(x)_j v_j, zeros where nothing is seen.
+ * Several tokens of one sequence in a call are rows of their own (each reads the cache).  head_dim is a multiple of 8, at most 256;
+ * pages, q and out start on 16 bytes and the strides are multiples of 16 bytes. */
+TL_API int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t* positions, const int32_t* token_seq, int64_t tokens,
+                                  const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t n_heads, void* out, float scale,
+                                  float softcap, int32_t window, const float* slopes);
+/* tl_sample: a token of each row of logits [rows, vocab] (row_stride elements apart) from given random numbers, out_tokens int32 [rows].
+ * The parameters are f32 (top_k: int32) [rows] on the device, each may be NULL (off).  A row's logits are divided by its temperature;
+ * of the vocabulary the top_k largest are kept (ties: the lowest indices; <= 0: all), of these, by size, the shortest
+ * prefix with top_p of their mass (>= 1: all; at least one), of these the ones with min_p times the largest's probability or more (<= 0: all).  The
+ * token is the first index at which the running mass of the kept ones, in the order of the vocabulary, exceeds uniforms[row] of their whole
+ * mass.  uniforms are in [0, 1); others are taken as the nearest, NaN as 0.  A temperature <= 0 or NaN, or uniforms NULL, gives the index of the
+ * largest logit, the lowest of equal ones.  NaN logits count as -infinity; a row without any other gives -1; logits of
+ * +infinity share the mass.  A NaN parameter is as off.  vocab is at most 2^24. */
+TL_API int32_t tl_sample(tl_ctx* ctx, const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride, const float* temperature,
+                         const int32_t* top_k, const float* top_p, const float* min_p, const float* uniforms, int32_t* out_tokens);
+
 /* ---- selection: planTiledMatmul / selectMatmulChoice / SelectionReceipt
  * (src/backend/webgpu/matmul/dispatch.ts:171-192, 1130-1329;
  *  src/backend/webgpu/matmul/variants.ts:54-260) ------------------------------ */

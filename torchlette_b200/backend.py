@@ -153,8 +153,41 @@ class CudaTensor:
 
 
 _NP_OF = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16, "u32": np.uint32, "u16": np.uint16,
-          "i8": np.int8}
+          "i8": np.int8, "i32": np.int32}
 _ITEMSIZE = {name: np.dtype(t).itemsize for name, t in _NP_OF.items()}  # np.dtype(...) and np.prod cost microseconds a call
+
+
+class PagedCache:
+    """A key-value cache whose sequences have their own lengths, on pages of their own: kPages and vPages [nPages, kvH, pageSize, D] and
+    pageTable i32 [nSeqs, maxPages], position p of a sequence in page pageTable[seq, p // pageSize] at p % pageSize.  The tensors stay the caller's
+    and their contents may change; entries behind a sequence's last page are not read.  A contiguous cache [B, kvH, capacity, D] is the case of
+    pageSize == capacity and a table [[0], [1], ...]."""
+
+    def __init__(self, backend, kPages: CudaTensor, vPages: CudaTensor, pageTable: CudaTensor):
+        if len(kPages.shape) != 4 or kPages.shape != vPages.shape or kPages.dtype != vPages.dtype or kPages.transposed or vPages.transposed:
+            raise TlError(B.TL_ERR_INVALID_ARG, "createPagedCache: kPages and vPages are [nPages, kvH, pageSize, D] of one dtype")
+        if kPages.dtype not in B.DTYPE_ID:
+            raise TlError(B.TL_ERR_INVALID_ARG, f"createPagedCache: pages of dtype {kPages.dtype}")
+        if len(pageTable.shape) != 2 or pageTable.dtype != "i32" or pageTable.transposed:
+            raise TlError(B.TL_ERR_INVALID_ARG, "createPagedCache: pageTable is i32 [nSeqs, maxPages]")
+        self.kPages, self.vPages, self.pageTable = kPages, vPages, pageTable
+        self.dtype = kPages.dtype
+        self.nPages, self.kvHeads, self.pageSize, self.headDim = kPages.shape
+        self.nSeqs, self.maxPages = pageTable.shape
+        self._shape = (self.nPages, self.pageSize, self.kvHeads, self.headDim, B.DTYPE_ID[self.dtype], self.nSeqs, self.maxPages)
+        self._bytes = self._at = None
+
+    def descriptor(self) -> bytes:
+        """The cache as the bytes of a tl_paged_cache."""
+        at = (self.kPages.buffer, self.vPages.buffer, self.pageTable.buffer)
+        if at != self._at:  # the first call, or a tensor was given another buffer
+            self._bytes, self._at = bytes(B.PagedCache(*at, *self._shape)), at
+        return self._bytes
+
+
+def _needs(ok: bool, message: str):
+    if not ok:
+        raise TlError(B.TL_ERR_INVALID_ARG, message)
 
 
 class CudaOps:
@@ -314,6 +347,109 @@ class CudaOps:
         esz = _ITEMSIZE[cache.dtype]
         self._b._calls.tl_copy2d(self._b._handle, cache.buffer + position * d * esz, cap * d * esz, new.buffer, d * esz, d * esz, b * kvh)
 
+    # -- a decode step over a paged cache (sequences of their own lengths) ----------
+    def _tokens(self, who: str, cache: PagedCache, positions: CudaTensor, tokenSeq: Optional[CudaTensor]) -> int:
+        _needs(positions.dtype == "i32" and len(positions.shape) == 1, f"{who}: positions are i32 [tokens]")
+        tokens = positions.shape[0]
+        _needs(tokenSeq is None or (tokenSeq.dtype == "i32" and tokenSeq.shape == [tokens]), f"{who}: tokenSeq is i32 [tokens]")
+        return tokens
+
+    def pagedAppend(self, cache: PagedCache, positions: CudaTensor, q: Optional[CudaTensor], k: Optional[CudaTensor], v: Optional[CudaTensor],
+                    cos: Optional[CudaTensor] = None, sin: Optional[CudaTensor] = None, *, qNorm: Optional[CudaTensor] = None,
+                    kNorm: Optional[CudaTensor] = None, eps: float = 1e-6, tokenSeq: Optional[CudaTensor] = None, headsFirst: bool = False,
+                    out: Optional[CudaTensor] = None) -> Optional[CudaTensor]:
+        """The per-head norms of q and k (qNorm, kNorm [D], where given), the rotation of fusedRoPE at each token's position (cos / sin f32
+        [rows, D/2], where given) and the append of k and v to the cache, in one launch; returns the new q [T, H, D].  q is [T, H, D] or
+        [T, H * D], k and v [T, kvH, D] or [T, kvH * D]; with ``headsFirst`` all of them, the result too, are [heads, T, D] (the order of
+        fusedRoPE and attention).  k = v = None: q holds the rows of one product, [T, (H + 2 kvH) * D].  q = None: k and v alone.
+        positions i32 [T], negative for tokens that are not there; tokenSeq i32 [T] their sequences (None: token t is of sequence t)."""
+        tokens, d, g = self._tokens("pagedAppend", cache, positions, tokenSeq), cache.headDim, cache.kvHeads
+        dtype, esz = cache.dtype, _ITEMSIZE[cache.dtype]
+        for t in (q, k, v, out):
+            _needs(t is None or (t.dtype == dtype and not t.transposed), "pagedAppend: q, k, v and out have the cache's dtype")
+        if k is None and v is None:
+            _needs(q is not None and not headsFirst and len(q.shape) == 2 and q.shape[0] == tokens and q.shape[1] % d == 0 and q.shape[1] > 2 * g * d,
+                   "pagedAppend: q alone is [tokens, (H + 2 kvH) * D]")
+            width = q.shape[1]
+            heads = width // d - 2 * g
+            q_at, k_at, v_at = q.buffer, q.buffer + heads * d * esz, q.buffer + (heads + g) * d * esz
+            strides = kv_strides = (width, d)
+        else:
+            _needs(k is not None and v is not None, "pagedAppend: k and v come together")
+            shapes = ([g, tokens, d],) if headsFirst else ([tokens, g, d], [tokens, g * d])
+            _needs(list(k.shape) in shapes and list(v.shape) in shapes, f"pagedAppend: k and v are {shapes[0]}")
+            kv_strides = (d, tokens * d) if headsFirst else (g * d, d)
+            k_at, v_at, q_at, heads, strides = k.buffer, v.buffer, None, 0, (0, 0)
+            if q is not None:
+                heads = q.shape[0] if headsFirst else int(math.prod(q.shape[1:])) // d
+                _needs(heads > 0 and list(q.shape) in (([heads, tokens, d],) if headsFirst else ([tokens, heads, d], [tokens, heads * d])),
+                       "pagedAppend: q is [tokens, H, D]")
+                q_at, strides = q.buffer, (d, tokens * d) if headsFirst else (heads * d, d)
+        for t in (qNorm, kNorm):
+            _needs(t is None or list(t.shape) == [d], "pagedAppend: qNorm and kNorm are [D]")
+        _needs(qNorm is None or kNorm is None or qNorm.dtype == kNorm.dtype, "pagedAppend: qNorm and kNorm have one dtype")
+        norm = qNorm if qNorm is not None else kNorm
+        _needs((cos is None) == (sin is None), "pagedAppend: cos and sin come together")
+        if cos is not None:
+            _needs(cos.dtype == sin.dtype == "f32" and len(cos.shape) == 2 and cos.shape == sin.shape and 2 * cos.shape[1] == d,
+                   "pagedAppend: cos and sin are f32 [rows, D/2]")
+        if q_at is None:
+            _needs(out is None, "pagedAppend: out is the new q's")
+        else:
+            shape = [heads, tokens, d] if headsFirst else [tokens, heads, d]
+            if out is None:
+                out = self.empty(shape, dtype)
+            else:
+                _needs(list(out.shape) in (shape, [tokens, heads * d] if not headsFirst else shape), "pagedAppend: out is q's shape")
+        out_strides = (d, tokens * d) if headsFirst else (heads * d, d)
+        self._b._calls.tl_paged_append(
+            self._b._handle, cache.descriptor(), positions.buffer, tokenSeq.buffer if tokenSeq is not None else None, tokens, q_at, *strides, heads,
+            out.buffer if out is not None else None, *out_strides, k_at, *kv_strides, v_at, *kv_strides,
+            qNorm.buffer if qNorm is not None else None, kNorm.buffer if kNorm is not None else None,
+            B.DTYPE_ID[norm.dtype] if norm is not None else 0, float(eps), cos.buffer if cos is not None else None,
+            sin.buffer if sin is not None else None, cos.shape[0] if cos is not None else 0)
+        return out
+
+    def pagedAttention(self, cache: PagedCache, positions: CudaTensor, q: CudaTensor, scale: float, *, softcap: float = 0.0, window: int = 0,
+                       slopes: Optional[CudaTensor] = None, tokenSeq: Optional[CudaTensor] = None, out: Optional[CudaTensor] = None) -> CudaTensor:
+        """softmax(cap(q k^T * scale) + slope * (j - p)) v of each token over its own sequence's positions j <= p (with ``window``: the last
+        ``window`` of them), p = positions[t] and among the appended ones.  q [T, H, D] or [T, H * D]; returns [T, H * D], the layout o_proj
+        reads, zeros for tokens that are not there (a negative position).  softcap 0: no cap; slopes f32 [H]; tokenSeq as in pagedAppend."""
+        tokens, d = self._tokens("pagedAttention", cache, positions, tokenSeq), cache.headDim
+        heads = int(math.prod(q.shape[1:])) // d
+        _needs(heads > 0 and list(q.shape) in ([tokens, heads, d], [tokens, heads * d]) and q.dtype == cache.dtype and not q.transposed,
+               "pagedAttention: q is [tokens, H, D] of the cache's dtype")
+        _needs(slopes is None or (slopes.dtype == "f32" and list(slopes.shape) == [heads]), "pagedAttention: slopes are f32 [H]")
+        if out is None:
+            out = self.empty([tokens, heads * d], cache.dtype)
+        else:
+            _needs(out.dtype == cache.dtype and not out.transposed and list(out.shape) in ([tokens, heads * d], [tokens, heads, d]),
+                   "pagedAttention: out is [tokens, H * D] of the cache's dtype")
+        self._b._calls.tl_paged_attention(self._b._handle, cache.descriptor(), positions.buffer, tokenSeq.buffer if tokenSeq is not None else None,
+                                          tokens, q.buffer, heads * d, d, heads, out.buffer, float(scale), float(softcap), int(window),
+                                          slopes.buffer if slopes is not None else None)
+        return out
+
+    def sample(self, logits: CudaTensor, uniforms: Optional[CudaTensor] = None, *, temperature: Optional[CudaTensor] = None,
+               topK: Optional[CudaTensor] = None, topP: Optional[CudaTensor] = None, minP: Optional[CudaTensor] = None,
+               out: Optional[CudaTensor] = None) -> CudaTensor:
+        """A token of each row of logits [rows, vocab] (any leading dims) from ``uniforms`` f32 [rows] in [0, 1): logits / temperature, the topK
+        largest, of these by size the shortest prefix with topP of their mass, of these the ones with minP times the largest's probability;
+        the first index whose running mass exceeds uniforms times the whole.  Each parameter is f32 (topK: i32) [rows] or None (off).
+        temperature <= 0, or no uniforms: the largest logit, the lowest index of equal ones.  -1 for a row that is all -infinity or NaN.
+        Returns i32 [rows]."""
+        _needs(len(logits.shape) >= 1 and not logits.transposed, "sample: logits are [rows, vocab]")
+        rows, vocab = int(math.prod(logits.shape[:-1])), logits.shape[-1]
+        for t, name, dtype in ((uniforms, "uniforms", "f32"), (temperature, "temperature", "f32"), (topK, "topK", "i32"), (topP, "topP", "f32"),
+                               (minP, "minP", "f32"), (out, "out", "i32")):
+            _needs(t is None or (t.dtype == dtype and list(t.shape) == [rows]), f"sample: {name} is {dtype} [rows]")
+        _needs(logits.dtype in B.DTYPE_ID, f"sample: logits of dtype {logits.dtype}")
+        if out is None:
+            out = self.empty([rows], "i32")
+        at = [t.buffer if t is not None else None for t in (temperature, topK, topP, minP, uniforms)]
+        self._b._calls.tl_sample(self._b._handle, logits.buffer, B.DTYPE_ID[logits.dtype], rows, vocab, vocab, *at, out.buffer)
+        return out
+
     def matmul(self, a: CudaTensor, b: CudaTensor, options: Optional[dict] = None) -> CudaTensor:
         """Backend matmul; the storage-format seam (matmul-ops.ts:42-59)."""
         if b.format is not None and b.format.packing is not None:
@@ -452,6 +588,10 @@ class CudaBackend:
         wt.format = format
         wt.scales = st
         return wt
+
+    def createPagedCache(self, kPages: CudaTensor, vPages: CudaTensor, pageTable: CudaTensor) -> PagedCache:
+        """The cache that pagedAppend fills and pagedAttention reads, over pages and a table that the caller owns."""
+        return PagedCache(self, kPages, vPages, pageTable)
 
     # -- descriptors ----------------------------------------------------------
     def _quant(self, packing: QuantPacking) -> bytes:

@@ -75,6 +75,11 @@ class PlanReceipt(C.Structure):
                 ("from_tuning_cache", C.c_int32), ("epilogue_engaged", C.c_int32)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_table", C.c_void_p), ("n_pages", C.c_int64), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32)]
+
+
 class Shape(C.Structure):
     _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64)]
 
@@ -125,6 +130,10 @@ SIGNATURES = {
     "tl_rope": (_I32, [_P, _P, _I32, _P, _P, _P, _I64, _I64, _I64, _F, _I64, _I64]),
     "tl_attention": (_I32, [_P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P, _I32]),
     "tl_decode_attention": (_I32, [_P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P]),
+    "tl_paged_append": (_I32, [_P, C.POINTER(PagedCache), _P, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
+                               _I32, _F, _P, _P, _I64]),
+    "tl_paged_attention": (_I32, [_P, C.POINTER(PagedCache), _P, _P, _I64, _P, _I64, _I64, _I64, _P, _F, _F, _I32, _P]),
+    "tl_sample": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P]),
     "tl_dequant_int8": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, C.POINTER(QuantDesc)]),
     "tl_unpack_int8": (_I32, [_P, _P, _P, _I64, _I64]),
     "tl_plan_qmatmul": (_I32, [_P, _I64, _I64, _I64, _I32, _I32, C.POINTER(QuantDesc), C.POINTER(Epilogue),
@@ -202,7 +211,7 @@ def load():
 
 
 CALLS = ("tl_alloc", "tl_free", "tl_copy2d", "tl_quantize_linear_weight_device", "tl_qmatmul_nt", "tl_matmul", "tl_unary_op", "tl_binary_op", "tl_rmsnorm",
-         "tl_rope", "tl_attention", "tl_decode_attention")
+         "tl_rope", "tl_attention", "tl_decode_attention", "tl_paged_append", "tl_paged_attention", "tl_sample")
 
 
 class _Calls:

@@ -566,6 +566,49 @@ FN(DecodeAttention) {
                                            (float)f64(env, argv[12]), (const float*)dptr(env, argv[13])));
 }
 
+/* a paged cache: { kPages, vPages, pageTable, nPages, pageSize, kvHeads, headDim, dtype, nSeqs, maxPages } */
+static int read_paged(napi_env env, napi_value o, tl_paged_cache* p) {
+  napi_value v;
+  if (type_of(env, o) != napi_object) { napi_throw_error(env, NULL, "tlcuda: a paged cache must be an object"); return 0; }
+  napi_get_named_property(env, o, "kPages", &v); p->k_pages = dptr(env, v);
+  napi_get_named_property(env, o, "vPages", &v); p->v_pages = dptr(env, v);
+  napi_get_named_property(env, o, "pageTable", &v); p->page_table = (const int32_t*)dptr(env, v);
+  napi_get_named_property(env, o, "nPages", &v); p->n_pages = i64(env, v);
+  napi_get_named_property(env, o, "pageSize", &v); p->page_size = i32(env, v);
+  napi_get_named_property(env, o, "kvHeads", &v); p->n_kv_heads = i32(env, v);
+  napi_get_named_property(env, o, "headDim", &v); p->head_dim = i32(env, v);
+  napi_get_named_property(env, o, "dtype", &v); p->dtype = i32(env, v);
+  napi_get_named_property(env, o, "nSeqs", &v); p->n_seqs = i32(env, v);
+  napi_get_named_property(env, o, "maxPages", &v); p->max_pages = i32(env, v);
+  return 1;
+}
+/* pagedAppend(ctx, cache, positions, tokenSeq | null, tokens, q | null, qTokenStride, qHeadStride, heads, qOut | null, outTokenStride, outHeadStride,
+ * k, kTokenStride, kHeadStride, v, vTokenStride, vHeadStride, qWeight | null, kWeight | null, weightDtype, eps, cos | null, sin | null, tableRows) */
+FN(PagedAppend) {
+  ARGS(25); CTX(0); tl_paged_cache p;
+  if (!read_paged(env, argv[1], &p)) return undef(env);
+  return check(env, c, tl_paged_append(c, &p, (const int32_t*)dptr(env, argv[2]), (const int32_t*)dptr(env, argv[3]), i64(env, argv[4]), dptr(env, argv[5]),
+                                       i64(env, argv[6]), i64(env, argv[7]), i64(env, argv[8]), dptr(env, argv[9]), i64(env, argv[10]), i64(env, argv[11]),
+                                       dptr(env, argv[12]), i64(env, argv[13]), i64(env, argv[14]), dptr(env, argv[15]), i64(env, argv[16]), i64(env, argv[17]),
+                                       dptr(env, argv[18]), dptr(env, argv[19]), i32(env, argv[20]), (float)f64(env, argv[21]),
+                                       (const float*)dptr(env, argv[22]), (const float*)dptr(env, argv[23]), i64(env, argv[24])));
+}
+/* pagedAttention(ctx, cache, positions, tokenSeq | null, tokens, q, qTokenStride, qHeadStride, heads, out, scale, softcap, window, slopes | null) */
+FN(PagedAttention) {
+  ARGS(14); CTX(0); tl_paged_cache p;
+  if (!read_paged(env, argv[1], &p)) return undef(env);
+  return check(env, c, tl_paged_attention(c, &p, (const int32_t*)dptr(env, argv[2]), (const int32_t*)dptr(env, argv[3]), i64(env, argv[4]), dptr(env, argv[5]),
+                                          i64(env, argv[6]), i64(env, argv[7]), i64(env, argv[8]), dptr(env, argv[9]), (float)f64(env, argv[10]),
+                                          (float)f64(env, argv[11]), i32(env, argv[12]), (const float*)dptr(env, argv[13])));
+}
+/* sample(ctx, logits, dtype, rows, vocab, rowStride, temperature | null, topK | null, topP | null, minP | null, uniforms | null, out) */
+FN(Sample) {
+  ARGS(12); CTX(0);
+  return check(env, c, tl_sample(c, dptr(env, argv[1]), i32(env, argv[2]), i64(env, argv[3]), i64(env, argv[4]), i64(env, argv[5]),
+                                 (const float*)dptr(env, argv[6]), (const int32_t*)dptr(env, argv[7]), (const float*)dptr(env, argv[8]),
+                                 (const float*)dptr(env, argv[9]), (const float*)dptr(env, argv[10]), (int32_t*)dptr(env, argv[11])));
+}
+
 /* attention(ctx, q, kCache, vCache, out, dtype, batch, heads, kvHeads, qLen, headDim, kvLen, kvCapacity, scale, mask | null, causal) */
 FN(Attention) {
   ARGS(16); CTX(0);
@@ -721,6 +764,7 @@ napi_value napi_register_module_v1(napi_env env, napi_value exports) {
       EXPORT("dequantInt8", DequantInt8), EXPORT("unpackInt8", UnpackInt8), EXPORT("quantizeLinearWeightInt4", QuantizeLinearWeightInt4),
       EXPORT("dequantInt4", DequantInt4), EXPORT("unpackInt4", UnpackInt4), EXPORT("matmul", Matmul),
       EXPORT("rmsnorm", Rmsnorm), EXPORT("rope", Rope), EXPORT("decodeAttention", DecodeAttention), EXPORT("attention", Attention),
+      EXPORT("pagedAppend", PagedAppend), EXPORT("pagedAttention", PagedAttention), EXPORT("sample", Sample),
       EXPORT("unaryOp", UnaryOp), EXPORT("binaryOp", BinaryOp), EXPORT("transpose2d", Transpose2d),
       EXPORT("planQmatmul", PlanQmatmul), EXPORT("variantName", VariantName), EXPORT("forceVariant", ForceVariant),
       EXPORT("classifyShape", ClassifyShape), EXPORT("shapeClassName", ShapeClassName),

@@ -178,8 +178,10 @@ int32_t tl_sync(tl_ctx* ctx) {
   TL_CHECK_CTX(ctx);
   DeviceGuard guard(ctx->device);
   TL_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-  int status = 0;
-  TL_CUDA(ctx, cudaMemcpy(&status, ctx->dev_status, sizeof(int), cudaMemcpyDeviceToHost));
+  int words[2] = {0, 0};
+  TL_CUDA(ctx, cudaMemcpy(words, ctx->dev_status, sizeof(words), cudaMemcpyDeviceToHost));
+  const int status = words[0];
+  if (words[1] != 0) cudaMemset(ctx->dev_status + 1, 0, sizeof(int));
   if (status != 0) {
     // a bounded device-side wait ran out: the scratch may hold partial sums, so clear it
     cudaMemset(ctx->dev_status, 0, sizeof(int));
@@ -188,6 +190,11 @@ int32_t tl_sync(tl_ctx* ctx) {
     if (ctx->stream_scratch) cudaMemset(ctx->stream_scratch, 0, size_t(ctx->sm_count) * (2 * 2 * 128 * sizeof(float) + sizeof(unsigned)));
     ctx->async_errors++;
     return tl_set_error(ctx, TL_ERR_TIMEOUT, "tl_sync: a kernel gave up a bounded wait (device code %d)", status);
+  }
+  if (words[1] != 0) {
+    ctx->async_errors++;
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_sync: a paged cache call skipped%s%s%s out of range", words[1] & kBadPosition ? " [a position]" : "",
+                        words[1] & kBadSequence ? " [a sequence]" : "", words[1] & kBadPage ? " [a page]" : "");
   }
   return TL_OK;
 }

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/tlcuda.h"
+#include "tl_paged.h"
 #include "tl_pool.cuh"
 
 // ---------------------------------------------------------------------------
@@ -60,6 +61,7 @@ struct tl_ctx {
   int live_graphs = 0;
   std::vector<std::pair<void*, size_t>> retired_scratch;
   int* dev_status = nullptr;  // written by kernels whose bounded waits ran out; read back by tl_sync
+                              // (word 1: kBad* bits of the paged cache's kernels, for indexes that only they can see)
   // drain-timed ring fill of the streaming GEMV (tl_qgemv_stream.cu): flag words on the device
   // and the slot the next launch takes; stream_scratch holds the partial sums and arrival
   // counters of row tiles that two CTAs share (fixed size, allocated once)
@@ -258,6 +260,9 @@ bool tl_lookup_tuned(tl_ctx* ctx, int64_t m, int64_t n, int64_t k, int32_t a_dty
 int32_t tl_check_qargs(tl_ctx* ctx, const char* who, const void* a, int32_t a_dtype,
                        const void* packed, const void* scales, const void* out, int32_t out_dtype,
                        int64_t m, int64_t n, int64_t k, const tl_quant_desc* q);
+
+// What a paged cache and the tokens of a call have to be; `who` names the call (tl_paged_append.cu).
+int32_t tl_check_paged(tl_ctx* ctx, const char* who, const tl_paged_cache* cache, const int32_t* positions, const int32_t* token_seq, int64_t tokens);
 
 // Launchers implemented by the kernel translation units.
 int32_t tl_launch_qgemv(tl_ctx* ctx, const tl_variant& v, const void* a, int32_t a_dtype,

@@ -1,0 +1,160 @@
+// Appending to a paged cache: the per-head norm of q and k, the rotation at each token's own position and the append of k and v, in one
+// launch where the separate ops take five (tl_rmsnorm and tl_rope for q and for k, a copy each for k and v with one position for all
+// sequences).
+//
+//   x^ = x * rsqrt(mean(x^2) + eps) * w;   y[d] = x^[d] c[d] - x^[d + D/2] s[d],  y[d + D/2] = x^[d + D/2] c[d] + x^[d] s[d]
+//
+// f32 arithmetic, one rounding at the store; v is copied bit for bit.
+#include <algorithm>
+
+#include "tl_vec.cuh"
+
+namespace {
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t qt, qh, ot, oh, kt, kh, vt, vh;  // strides in elements: tokens, heads
+  void *k_pages, *v_pages;
+  const int32_t *page_table, *positions, *token_seq;
+  const void *q_weight, *k_weight;
+  const float *cos_t, *sin_t;
+  int64_t tokens, table_rows, n_pages;
+  int32_t n_heads, n_kv_heads, head_dim, page_size, n_seqs, max_pages, dtype, w_dtype;
+  float eps;
+  int* status;
+};
+
+// Where token t goes: false if it is not there.  `at`: its element offset in k_pages and v_pages, of head 0, or -1 if its page is not there.
+__device__ __forceinline__ bool place(const AppendArgs& p, int64_t t, int& pos, int64_t& at) {
+  pos = p.positions[t];
+  if (pos < 0) return false;
+  const int64_t seq = p.token_seq ? int64_t(p.token_seq[t]) : t;
+  const int bad = tl_bad_token(pos, seq, p.n_seqs, p.max_pages, p.page_size, p.cos_t ? p.table_rows : -1);
+  if (bad) { atomicOr(p.status, bad); return false; }
+  const int index = pos / p.page_size, page = p.page_table[seq * p.max_pages + index];
+  at = -1;
+  if (tl_bad_page(page, p.n_pages)) atomicOr(p.status, kBadPage);
+  else at = tl_page_at(page, pos - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim);
+  return true;
+}
+
+// Any strides and even head_dim: a warp per token and head (q's, then k's, then v's), a lane per pair of dimensions.
+__global__ void __launch_bounds__(128) append_kernel(AppendArgs p) {
+  tl_pdl_wait();
+  const int lane = threadIdx.x & 31, half = p.head_dim >> 1;
+  const int rows = (p.q ? p.n_heads : 0) + 2 * p.n_kv_heads;
+  const int64_t all = p.tokens * rows, step = int64_t(gridDim.x) * 4;
+  for (int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5); w < all; w += step) {
+    const int64_t t = w / rows;
+    int r = int(w - t * rows), pos;
+    int64_t at;
+    if (!place(p, t, pos, at)) continue;
+    const void *x, *weight;
+    void* y;
+    int64_t xi, yi;
+    if (p.q && r < p.n_heads) {
+      x = p.q; y = p.q_out; weight = p.q_weight;
+      xi = t * p.qt + r * p.qh; yi = t * p.ot + r * p.oh;
+    } else {
+      if (p.q) r -= p.n_heads;
+      if (at < 0) continue;
+      const bool is_k = r < p.n_kv_heads;
+      if (!is_k) r -= p.n_kv_heads;
+      x = is_k ? p.k : p.v; y = is_k ? p.k_pages : p.v_pages; weight = p.k_weight;
+      xi = is_k ? t * p.kt + r * p.kh : t * p.vt + r * p.vh;
+      yi = at + int64_t(r) * p.page_size * p.head_dim;
+      if (!is_k) {
+        for (int d = lane; d < p.head_dim; d += 32) tl_store_out(y, p.dtype, yi + d, ld_f32(x, p.dtype, xi + d));
+        continue;
+      }
+    }
+    float inv = 1.f;
+    if (weight) {
+      float ss = 0.f;
+      for (int d = lane; d < p.head_dim; d += 32) {
+        const float e = ld_f32(x, p.dtype, xi + d);
+        ss = fmaf(e, e, ss);
+      }
+      inv = rsqrtf(warp_sum(ss) / float(p.head_dim) + p.eps);
+      __syncwarp();
+    }
+    for (int d = lane; d < half; d += 32) {
+      float a = ld_f32(x, p.dtype, xi + d), b = ld_f32(x, p.dtype, xi + d + half);
+      if (weight) {
+        a = a * inv * ld_f32(weight, p.w_dtype, d);
+        b = b * inv * ld_f32(weight, p.w_dtype, d + half);
+      }
+      float c = 1.f, s = 0.f;
+      if (p.cos_t) { c = p.cos_t[int64_t(pos) * half + d]; s = p.sin_t[int64_t(pos) * half + d]; }
+      tl_store_out(y, p.dtype, yi + d, a * c - b * s);
+      tl_store_out(y, p.dtype, yi + d + half, b * c + a * s);
+    }
+  }
+}
+
+}  // namespace
+
+int32_t tl_check_paged(tl_ctx* ctx, const char* who, const tl_paged_cache* c, const int32_t* positions, const int32_t* token_seq, int64_t tokens) {
+  if (!c) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "%s: null cache", who);
+  if (c->n_pages < 0 || c->page_size < 1 || c->n_kv_heads < 1 || c->head_dim < 1 || c->n_seqs < 0 || c->max_pages < 0 || tokens < 0)
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "%s: bad shape (pages %lld of %d, kv heads %d, head dim %d, sequences %d of %d pages, tokens %lld)", who,
+                        (long long)c->n_pages, c->page_size, c->n_kv_heads, c->head_dim, c->n_seqs, c->max_pages, (long long)tokens);
+  if (!tl_dtype_valid(c->dtype)) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "%s: unknown dtype", who);
+  if (tokens == 0) return TL_OK;
+  if (!positions || !c->k_pages || !c->v_pages || !c->page_table) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!token_seq && tokens > c->n_seqs)
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "%s: %lld tokens for %d sequences need token_seq", who, (long long)tokens, c->n_seqs);
+  // positions are int32, and an offset inside a page too
+  if (int64_t(c->max_pages) * c->page_size > INT32_MAX || int64_t(c->n_kv_heads) * c->page_size * c->head_dim > INT32_MAX || tokens > INT32_MAX)
+    return tl_set_error(ctx, TL_ERR_UNSUPPORTED, "%s: positions, a page's elements and tokens are limited to 2^31 - 1", who);
+  return TL_OK;
+}
+
+extern "C" {
+
+int32_t tl_paged_append(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t* positions, const int32_t* token_seq, int64_t tokens, const void* q,
+                        int64_t q_token_stride, int64_t q_head_stride, int64_t n_heads, void* q_out, int64_t out_token_stride, int64_t out_head_stride,
+                        const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                        const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps, const float* cos_table, const float* sin_table,
+                        int64_t table_rows) {
+  TL_CHECK_CTX(ctx);
+  int32_t rc = tl_check_paged(ctx, "tl_paged_append", cache, positions, token_seq, tokens);
+  if (rc != TL_OK) return rc;
+  if (cache->head_dim % 2 != 0 || cache->head_dim > 1024)
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_append: head_dim must be even and at most 1024, got %d", cache->head_dim);
+  if ((q_weight || k_weight) && !tl_dtype_valid(weight_dtype)) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_append: unknown weight dtype");
+  if (!cos_table != !sin_table || (cos_table && table_rows < 0))
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_append: the rotation needs both tables and their rows");
+  if (q && (n_heads < 1 || n_heads > 65535)) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_append: bad n_heads %lld", (long long)n_heads);
+  if (tokens == 0) return TL_OK;
+  if (!k || !v || !q != !q_out) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_append: null k or v, or only one of q and q_out");
+  if (q == q_out && q && (q_token_stride != out_token_stride || q_head_stride != out_head_stride))
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_append: in place q_out has q's strides");
+  if ((q && (q_token_stride < 0 || q_head_stride < 0 || out_token_stride < 0 || out_head_stride < 0)) || k_token_stride < 0 || k_head_stride < 0 ||
+      v_token_stride < 0 || v_head_stride < 0)
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_append: negative stride");
+  DeviceGuard guard(ctx->device);
+  AppendArgs p{};
+  p.q = q; p.k = k; p.v = v; p.q_out = q_out;
+  p.qt = q_token_stride; p.qh = q_head_stride; p.ot = out_token_stride; p.oh = out_head_stride;
+  p.kt = k_token_stride; p.kh = k_head_stride; p.vt = v_token_stride; p.vh = v_head_stride;
+  p.k_pages = cache->k_pages; p.v_pages = cache->v_pages; p.page_table = cache->page_table; p.positions = positions; p.token_seq = token_seq;
+  p.q_weight = q_weight; p.k_weight = k_weight; p.cos_t = cos_table; p.sin_t = sin_table;
+  p.tokens = tokens; p.table_rows = table_rows; p.n_pages = cache->n_pages;
+  p.n_heads = int32_t(n_heads); p.n_kv_heads = cache->n_kv_heads; p.head_dim = cache->head_dim; p.page_size = cache->page_size;
+  p.n_seqs = cache->n_seqs; p.max_pages = cache->max_pages; p.dtype = cache->dtype; p.w_dtype = weight_dtype;
+  p.eps = eps; p.status = ctx->dev_status + 1;
+  const int64_t rows = tokens * ((q ? n_heads : 0) + 2 * int64_t(cache->n_kv_heads));
+  const int64_t grid = std::min<int64_t>((rows + 3) / 4, int64_t(ctx->sm_count) * 16);
+  TL_CUDA(ctx, tl_launch_waiting(append_kernel, dim3(unsigned(grid)), dim3(128), ctx->stream, p));
+  ctx->counters[TL_COUNTER_KERNEL_LAUNCHES]++;
+  const int64_t page_bytes = cache->n_pages * cache->n_kv_heads * cache->page_size * cache->head_dim * int64_t(tl_dtype_size(cache->dtype));
+  tl_wrote(ctx, cache->k_pages, page_bytes, true);
+  tl_wrote(ctx, cache->v_pages, page_bytes);
+  if (q_out)
+    tl_wrote(ctx, q_out, ((tokens - 1) * out_token_stride + (n_heads - 1) * out_head_stride + cache->head_dim) * int64_t(tl_dtype_size(cache->dtype)));
+  return TL_OK;
+}
+
+}  // extern "C"

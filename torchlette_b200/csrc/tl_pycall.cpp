@@ -26,7 +26,7 @@ template <typename T> bool convert(PyObject* o, T* out) {
     if (o == Py_None) { *out = nullptr; return true; }
     if (PyLong_Check(o)) { *out = reinterpret_cast<T>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLongMask(o))); return true; }
     using Pointee = std::remove_const_t<std::remove_pointer_t<T>>;
-    if constexpr (std::is_same_v<Pointee, tl_quant_desc> || std::is_same_v<Pointee, tl_epilogue>) {
+    if constexpr (std::is_same_v<Pointee, tl_quant_desc> || std::is_same_v<Pointee, tl_epilogue> || std::is_same_v<Pointee, tl_paged_cache>) {
       if (PyBytes_CheckExact(o) && PyBytes_GET_SIZE(o) == Py_ssize_t(sizeof(Pointee))) { *out = reinterpret_cast<T>(PyBytes_AS_STRING(o)); return true; }
     }
     return false;
@@ -72,7 +72,8 @@ struct Entry { const char* name; Thunk thunk; Py_ssize_t args; };
 const Entry kEntries[] = {TL_ENTRY(tl_free),     TL_ENTRY(tl_copy2d),    TL_ENTRY(tl_quantize_linear_weight_device),
                           TL_ENTRY(tl_qmatmul_nt), TL_ENTRY(tl_matmul),  TL_ENTRY(tl_unary_op),
                           TL_ENTRY(tl_binary_op), TL_ENTRY(tl_rmsnorm),  TL_ENTRY(tl_rope),
-                          TL_ENTRY(tl_attention), TL_ENTRY(tl_decode_attention)};
+                          TL_ENTRY(tl_attention), TL_ENTRY(tl_decode_attention), TL_ENTRY(tl_paged_append),
+                          TL_ENTRY(tl_paged_attention), TL_ENTRY(tl_sample)};
 
 struct Bound {
   PyObject_HEAD

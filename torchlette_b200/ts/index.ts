@@ -37,7 +37,7 @@ let ctx: Handle | null = null;
 let initError: string | null = null;
 
 const DTYPE_ID: Record<string, number> = { f32: 0, f16: 1, bf16: 2 };
-const DTYPE_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2, u32: 4, u16: 2, i8: 1 };
+const DTYPE_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2, u32: 4, u16: 2, i8: 1, i32: 4 };
 const UNARY: Record<string, number> = { relu: 1, silu: 2, sigmoid: 3, tanh: 4, gelu: 5, gelu_tanh: 5, gelu_erf: 6 };
 const BINARY: Record<string, number> = { add: 1, sub: 2, mul: 3 };
 const COUNTER = { qgemv: 0, dequant: 1, gemvEpilogue: 2, qgemm: 3, launches: 4, gemv: 5, tiled: 6 } as const;
@@ -106,9 +106,10 @@ export function empty(shape: number[], dtype: string): CudaTensor {
   const nbytes = numel(shape) * DTYPE_BYTES[dtype];
   return makeTensor(shape, dtype, addon.alloc(need(), nbytes), nbytes);
 }
-function hostArrayFor(t: CudaTensor): Float32Array | Uint16Array | Uint32Array | Int8Array {
+function hostArrayFor(t: CudaTensor): Float32Array | Uint16Array | Uint32Array | Int32Array | Int8Array {
   const n = numel(t.shape);
-  return t.dtype === "f32" ? new Float32Array(n) : t.dtype === "u32" ? new Uint32Array(n) : t.dtype === "i8" ? new Int8Array(n) : new Uint16Array(n);
+  return t.dtype === "f32" ? new Float32Array(n) : t.dtype === "u32" ? new Uint32Array(n) : t.dtype === "i8" ? new Int8Array(n)
+    : t.dtype === "i32" ? new Int32Array(n) : new Uint16Array(n);
 }
 /** Blocking read (tests, toArray). */
 export function readSync(t: CudaTensor) {
@@ -206,6 +207,47 @@ export function attention(q: CudaTensor, kCache: CudaTensor, vCache: CudaTensor,
   const out = empty([b, s, h * d], q.dtype as string);
   addon.attention(need(), q.buffer, kCache.buffer, vCache.buffer, out.buffer, DTYPE_ID[q.dtype as string], b, h, kCache.shape[1], s, d, kvLen,
                   kCache.shape[2], scale, mask ? mask.buffer : null, causal ? 1 : 0);
+  return out;
+}
+
+// ---- a decode step over a paged cache (no counterpart in the reference): sequences of their own lengths ------------
+/** kPages, vPages [nPages, kvH, pageSize, D] and pageTable i32 [nSeqs, maxPages]; position p of a sequence lies in page
+ * pageTable[seq][p / pageSize] at p % pageSize.  A contiguous cache [B, kvH, capacity, D] has pageSize == capacity and a table [[0], [1], ...]. */
+export interface PagedCache { kPages: CudaTensor; vPages: CudaTensor; pageTable: CudaTensor }
+const pagedArg = (c: PagedCache): any => ({
+  kPages: c.kPages.buffer, vPages: c.vPages.buffer, pageTable: c.pageTable.buffer, nPages: c.kPages.shape[0], kvHeads: c.kPages.shape[1],
+  pageSize: c.kPages.shape[2], headDim: c.kPages.shape[3], dtype: DTYPE_ID[c.kPages.dtype as string], nSeqs: c.pageTable.shape[0],
+  maxPages: c.pageTable.shape[1],
+});
+/** The per-head norms of q and k, the rotation at each token's position and the append of k and v, one launch; the new q [T, H, D].
+ * q [T, H, D], k and v [T, kvH, D]; positions i32 [T] (negative: not there), tokenSeq i32 [T] (absent: token t is of sequence t). */
+export function pagedAppend(cache: PagedCache, positions: CudaTensor, q: CudaTensor, k: CudaTensor, v: CudaTensor,
+                            config: { cos?: CudaTensor; sin?: CudaTensor; qNorm?: CudaTensor; kNorm?: CudaTensor; eps?: number;
+                                      tokenSeq?: CudaTensor } = {}): CudaTensor {
+  const p = pagedArg(cache), d = p.headDim, g = p.kvHeads, tokens = positions.shape[0], heads = numel(q.shape) / (tokens * d);
+  const out = empty([tokens, heads, d], q.dtype as string), norm = config.qNorm ?? config.kNorm;
+  const at = (t?: CudaTensor): any => (t ? t.buffer : null);
+  addon.pagedAppend(need(), p, positions.buffer, at(config.tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, heads * d, d, k.buffer, g * d, d,
+                    v.buffer, g * d, d, at(config.qNorm), at(config.kNorm), norm ? DTYPE_ID[norm.dtype as string] : 0, config.eps ?? 1e-6,
+                    at(config.cos), at(config.sin), config.cos ? config.cos.shape[0] : 0);
+  return out;
+}
+/** Attention of each token over its own sequence's positions up to its own: q [T, H, D] -> [T, H * D]. */
+export function pagedAttention(cache: PagedCache, positions: CudaTensor, q: CudaTensor, scale: number,
+                               config: { softcap?: number; window?: number; slopes?: CudaTensor; tokenSeq?: CudaTensor } = {}): CudaTensor {
+  const p = pagedArg(cache), d = p.headDim, tokens = positions.shape[0], heads = numel(q.shape) / (tokens * d);
+  const out = empty([tokens, heads * d], q.dtype as string);
+  addon.pagedAttention(need(), p, positions.buffer, config.tokenSeq ? config.tokenSeq.buffer : null, tokens, q.buffer, heads * d, d, heads, out.buffer,
+                       scale, config.softcap ?? 0, config.window ?? 0, config.slopes ? config.slopes.buffer : null);
+  return out;
+}
+/** A token of each row of logits [rows, vocab] from uniforms f32 [rows]; parameters f32 (topK: i32) [rows] or absent.  Returns i32 [rows]. */
+export function sample(logits: CudaTensor, uniforms: CudaTensor | null,
+                       config: { temperature?: CudaTensor; topK?: CudaTensor; topP?: CudaTensor; minP?: CudaTensor } = {}): CudaTensor {
+  const vocab = logits.shape[logits.shape.length - 1], rows = numel(logits.shape) / vocab, out = empty([rows], "i32");
+  const at = (t?: CudaTensor | null): any => (t ? t.buffer : null);
+  addon.sample(need(), logits.buffer, DTYPE_ID[logits.dtype as string], rows, vocab, vocab, at(config.temperature), at(config.topK), at(config.topP),
+               at(config.minP), at(uniforms), out.buffer);
   return out;
 }
 
