@@ -14,3 +14,20 @@ extern "C" int stub_bad_token(int pos, long long seq, int n_seqs, int max_pages,
 }
 extern "C" int stub_bad_page(int page, long long n_pages) { return tl_bad_page(page, n_pages); }
 extern "C" long long stub_page_at(int page, int slot, int heads, int page_size, int dim) { return tl_page_at(page, slot, heads, page_size, dim); }
+extern "C" int stub_units(int first, int end, int keys) { return tl_units(first, end, keys); }
+extern "C" long long stub_share_begin(long long units, int ctas, int cta) { return tl_share_begin(units, ctas, cta); }
+extern "C" int stub_share_owner(long long units, int ctas, long long unit) { return tl_share_owner(units, ctas, unit); }
+extern "C" int stub_share_ctas(long long units, int most, int least) { return tl_share_ctas(units, most, least); }
+// The first n at which the quotient by d is wrong, of `count` neighbours of every multiple that is tried; -1: none
+extern "C" long long stub_divide_wrong(int d, int tries) {
+  const TlDivide by = tl_divide_by(d);
+  const long long most = 2147483647;
+  for (int i = 0; i <= tries; ++i) {
+    const long long m = most / d * i / tries * d;
+    for (long long n = m - 2; n <= m + 2; ++n)
+      if (n >= 0 && n <= most && tl_divide(int(n), by) != n / d) return n;
+  }
+  for (long long n = most - 2 * (long long)(d); n <= most; n += d > 1000 ? d / 500 : 1)
+    if (n >= 0 && tl_divide(int(n), by) != n / d) return n;
+  return -1;
+}

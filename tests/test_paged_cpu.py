@@ -25,6 +25,10 @@ def stub(tmp_path_factory):
     lib.stub_bad_page.argtypes = [C.c_int, C.c_longlong]
     lib.stub_page_at.argtypes = [C.c_int] * 5
     lib.stub_page_at.restype = C.c_longlong
+    for name, kinds, result in (("share_begin", [C.c_longlong, C.c_int, C.c_int], C.c_longlong), ("share_owner", [C.c_longlong, C.c_int, C.c_longlong], C.c_int),
+                                ("share_ctas", [C.c_longlong, C.c_int, C.c_int], C.c_int), ("divide_wrong", [C.c_int, C.c_int], C.c_longlong)):
+        f = getattr(lib, "stub_" + name)
+        f.argtypes, f.restype = kinds, result
     return lib
 
 
@@ -145,6 +149,50 @@ def test_only_indexes_in_range_become_addresses(stub):
         assert at == ((page * heads) * page_size + slot) * dim and 0 <= at and at + ((heads - 1) * page_size + 1) * dim <= size
     # offsets past 2^31
     assert stub.stub_page_at(big, 15, 8, 16, 128) == (big * 8 * 16 + 15) * 128
+
+
+def test_every_unit_has_one_owner(stub):
+    """The shares cover the units without gaps, none is empty, and the owner of a unit is the CTA whose share holds it."""
+    for units, most, least in itertools.product([1, 2, 3, 4, 5, 37, 295, 296, 297, 1000, 40_001], [1, 2, 148, 296], [1, 4]):
+        ctas = stub.stub_share_ctas(units, most, least)
+        assert 1 <= ctas <= most and (ctas == most or ctas * least >= units) and ctas <= units
+        begins = [stub.stub_share_begin(units, ctas, c) for c in range(ctas + 1)]
+        assert begins[0] == 0 and begins[-1] == units and all(a < b for a, b in zip(begins, begins[1:]))
+        for c in range(ctas):
+            assert stub.stub_share_owner(units, ctas, begins[c]) == c and stub.stub_share_owner(units, ctas, begins[c + 1] - 1) == c
+    big = (1 << 40) + 12345  # units of a call at the limits
+    for c in range(296):
+        assert stub.stub_share_owner(big, 296, stub.stub_share_begin(big, 296, c)) == c
+    assert [stub.stub_units(a, b, 64) for a, b in ((0, 0), (5, 5), (0, 1), (0, 64), (0, 65), (3, 67), (2 ** 31 - 66, 2 ** 31 - 1))] == [0, 0, 1, 1, 2, 1, 2]
+
+
+def test_parts_of_a_token_meet_in_slots_of_their_own(stub):
+    """Walked on the host: each CTA leaves at most one part in each of its two slots, the CTAs between a token's first and last owner are those that leave one, and
+    no two tokens' groups of sixteen count their arrivals in the same place."""
+    for lengths, ctas in (([1, 7, 300, 2, 2, 90], 37), ([5000], 296), ([33] * 50, 296), ([1000, 1, 1, 999], 296)):
+        units = sum(lengths)
+        parts, places, at = {}, set(), 0
+        for n in lengths:
+            first, last = (stub.stub_share_owner(units, ctas, u) for u in (at, at + n - 1))
+            for c in range(first, last + 1):
+                begin, end = (stub.stub_share_begin(units, ctas, x) for x in (c, c + 1))
+                assert begin < at + n and end > at  # it has some of the token
+                starts = at >= begin
+                assert starts == (c == first)
+                if first != last:
+                    slot = 2 * c + starts
+                    assert slot not in parts
+                    parts[slot] = at
+                    if (c - first) % 16 == 0:
+                        place = 2 * c + (c == first)
+                        assert place not in places and place < 2 * ctas
+                        places.add(place)
+            at += n
+
+
+@pytest.mark.parametrize("d", [1, 2, 3, 5, 7, 16, 24, 48, 100, 255, 256, 257, 641, 65_535, 65_537, 1_000_003, 2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1])
+def test_division_by_the_page_size(stub, d):
+    assert stub.stub_divide_wrong(d, 5000) == -1
 
 
 # ---- the backend's own checks, and what it hands over ----------------------------------------------------------------------

@@ -165,6 +165,7 @@ int32_t tl_ctx_destroy(tl_ctx* ctx) {
   for (auto& p : ctx->retired_scratch) cudaFree(p.first);
   if (ctx->dev_status) cudaFree(ctx->dev_status);
   if (ctx->stream_scratch) cudaFree(ctx->stream_scratch);
+  if (ctx->paged_scratch) cudaFree(ctx->paged_scratch);
   if (ctx->prof_e0) { cudaEventDestroy(ctx->prof_e0); cudaEventDestroy(ctx->prof_e1); }
   for (int r = 0; r < tl_ctx::kMaxPeers; ++r)
     if (ctx->p2p_peer[r] && ctx->p2p_peer[r] != ctx->p2p_local) cudaIpcCloseMemHandle(ctx->p2p_peer[r]);
