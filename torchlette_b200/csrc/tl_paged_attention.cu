@@ -4,28 +4,35 @@
 //
 // in one pass over the keys, with the running maximum m, sum and output of the softmax in f32 registers.  Bound: HBM, the cache is read once.
 //
-// Work.  The keys of all tokens are cut into units (64 keys of one token and one KV head's query heads), and the units dealt out to
+// Work.  The keys of all tokens are cut into tiles (16 of one token and one KV head's query heads, f32 8), and the tiles dealt out to
 // a fixed number of resident CTAs in equal contiguous shares (tl_paged.h): sequences of any lengths load all SMs alike, and nothing on the host
-// depends on a length, so that a captured call serves sequences that grow.  A warp takes 16 keys of every unit, for which it keeps a ring of its
-// own in shared memory, filled by cp.async a few units ahead across the borders of tokens and heads: no barrier inside a token's keys.
-// Where a share ends inside a token's keys the CTA leaves maximum, sum and output in scratch, and whoever of that token's CTAs comes last
-// joins them in the order of the keys (in groups of 16 first, where they are many), so that no result depends on timing.
+// depends on a length, so that a captured call serves sequences that grow.  A producer warp looks up the pages, a batch of tiles ahead, and fills a ring of tiles
+// in shared memory across the borders of tokens and heads; four consumer warps take the tiles in turn, each with a softmax of its own, and
+// meet at the end of a token's keys.  Where a share ends inside a token's keys the CTA leaves maximum, sum and output in scratch, and whoever of that
+// token's CTAs comes last joins them in the order of the keys (in groups of 16 first, where they are many), so that no result depends on timing.
+//
+// The ring.  Where a tile's rows are neighbours in a page (page_size a multiple of the tile), TMA boxes of 128-byte columns, 128-byte swizzle: an
+// instruction for each 2 KB.  Other page sizes: cp.async into the same layout, 16 bytes a lane.
+// (A ring of each warp's own, filled by its own cp.async, was 63 us on 8 sequences x 8 KV heads x 4000 keys x 128 f16: 700 instructions a tile, most of
+// them addresses, and a wait for the page table in every one.)
 //
 // f16 / bf16.  The rows of a tile are the A operand of S^T = K q^T (ldmatrix) and, transposed on the way, of O^T = V^T p; the probabilities go
 // from accumulators to the B operand in the register file (movmatrix), split into 16-bit terms that keep nearly all bits (tl_attention.cuh).
 // f32: CUDA cores, a lane per D / 32 dimensions; the partial dot products of eight keys are summed over the lanes by exchanging halves.
 //
-// Keys that no token sees are not read: rows of a tile past a token's end are zero-filled by the copy, whatever the pages hold there.
+// Rows of a tile that the token does not see never count: their scores are replaced, not multiplied, and their values zeroed before the
+// product, whatever the pages hold there.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
 
 #include "tl_attention.cuh"
 #include "tl_mma_frag.cuh"
+#include "tl_tma.cuh"
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kGroup = 16;
+constexpr int kWarps = 4, kConsumers = 32 * kWarps, kThreads = kConsumers + 32, kGroup = 16, kMaxStages = 24;
 
 struct PagedArgs {
   const void *q, *k_pages, *v_pages;
@@ -33,20 +40,22 @@ struct PagedArgs {
   const int32_t *page_table, *positions, *token_seq;
   const float* slopes;
   int64_t qt, qh, n_pages;
-  int32_t tokens, n_heads, n_kv_heads, rep, head_dim, page_size, n_seqs, max_pages, window, row_tiles, least_units;
+  int32_t tokens, n_heads, n_kv_heads, rep, head_dim, page_size, n_seqs, max_pages, window, row_tiles, least_units, stages;
   TlDivide page_div;
   float scale, softcap;
-  int* status;
+  int *status, *wait_status;
   float* slots;        // [2 * CTAs] parts of tokens
   unsigned* arrivals;  // [3 * CTAs], zero between launches: CTAs of a group that have left their part, groups of a token
 };
 
-__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {  // 16 bytes, or zeros with bytes == 0
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Arrives once this thread's copies so far have landed
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
 __device__ __forceinline__ void ldmatrix4(uint32_t at, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
@@ -79,20 +88,21 @@ __device__ __forceinline__ Token token_of(const PagedArgs& p, int t, bool report
   return k;
 }
 
-// A place in the call's units: unit `u` of the `n` of token t and its group `seg` = (KV head, tile of its query heads)
+// A place in the call's tiles: tile `u` of the `n` of token t and its group `seg` = (KV head, tile of its query heads).  Tiles lie at multiples of
+// KEYS in the sequence.
 struct Cursor {
   int t, seg, u, n, kvh, tile;
   Token k;
   template <int KEYS> __device__ __forceinline__ void open(const PagedArgs& p) {
     k = token_of(p, t, false);
-    n = tl_units(k.lo, k.hi, KEYS);
+    n = tl_units(k.lo / KEYS * KEYS, k.hi, KEYS);
   }
   __device__ __forceinline__ void head(const PagedArgs& p) {
     if (p.row_tiles == 1) { kvh = seg; tile = 0; }
     else { kvh = seg / p.row_tiles; tile = seg - kvh * p.row_tiles; }
   }
+  // from u == n to the next group's first tile
   template <int KEYS> __device__ __forceinline__ void next(const PagedArgs& p) {
-    if (++u < n) return;
     u = 0;
     if (++seg == p.n_kv_heads * p.row_tiles) {
       seg = 0;
@@ -103,6 +113,7 @@ struct Cursor {
     }
     head(p);
   }
+  template <int KEYS> __device__ __forceinline__ int first_key(int i) const { return (k.lo / KEYS + i) * KEYS; }
 };
 
 // One row again, by one warp and over exactly the keys that it sees: its result is not finite, and whether that is what the cache holds or an infinite value times
@@ -145,16 +156,13 @@ template <> constexpr float kProbBias<__half> = 10.f;
 
 // What a warp holds of the softmax of its keys, and how it takes a tile of them in: 16-bit types on the tensor cores.
 // NT = 1: up to 8 query heads of a KV head, NT = 2: up to 16.
-template <typename AT_, int DPAD_, int NT, int STAGES_>
+template <typename AT_, int DPAD_, int NT>
 struct MmaTile {
   using AT = AT_;
-  static constexpr int DPAD = DPAD_, ROWS = 8 * NT, KEYS = 16, STAGES = STAGES_, CHUNKS = DPAD / 8, TERMS = ProbSplit<AT>::kTerms;
+  static constexpr int DPAD = DPAD_, ROWS = 8 * NT, KEYS = 16, TERMS = ProbSplit<AT>::kTerms, CTAS = DPAD * NT > 128 ? 1 : 2;
   static constexpr bool kRedo = true;  // infinite values need it
   uint32_t q[NT][DPAD / 16][2];
   float o[NT][DPAD / 16][4], m[NT][2], l[NT][2], slope[NT][2];
-
-  // chunk c of row r, 16 bytes each, so that the eight rows that ldmatrix reads at once lie in different banks
-  static __device__ __forceinline__ int chunk_at(int r, int c) { return r * CHUNKS + (c ^ (r & 7)); }
 
   __device__ __forceinline__ void begin(const PagedArgs& p, int t, int kvh, int tile) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -186,6 +194,7 @@ struct MmaTile {
     float s[NT][4];
     {
       const int r = (lane & 7) + ((lane >> 3) & 1) * 8, half = lane >> 4;
+      const uint32_t at = ks + 128 * r, x = ((r & 7) ^ half) << 4;  // 16-byte chunk 2 i + half of row r, swizzled
       float s0[NT][4], s1[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -194,7 +203,7 @@ struct MmaTile {
 #pragma unroll
       for (int i = 0; i < DPAD / 16; ++i) {
         uint32_t a[4];
-        ldmatrix4(ks + 16 * chunk_at(r, 2 * i + half), a);
+        ldmatrix4(at + (i >> 2) * (KEYS * 128) + (x ^ ((2 * (i & 3)) << 4)), a);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) MmaOps<AT>::mma_free(i & 1 ? s1[nt] : s0[nt], a[0], a[1], a[2], a[3], q[nt][i][0], q[nt][i][1]);
       }
@@ -218,7 +227,7 @@ struct MmaTile {
         } else {
           x = s[nt][e] * (p.scale * kLog2e);
         }
-        s[nt][e] = (seen >> key) & 1 ? x : -INFINITY;
+        s[nt][e] = seen == 0xffffu || (seen >> key) & 1 ? x : -INFINITY;
       }
       float nm[2];
 #pragma unroll
@@ -259,10 +268,11 @@ struct MmaTile {
       }
     }
     const int r = (lane & 7) + (lane >> 4) * 8, half = (lane >> 3) & 1;
+    const uint32_t at = vs + 128 * r, x = ((r & 7) ^ half) << 4;
 #pragma unroll
     for (int i = 0; i < DPAD / 16; ++i) {
       uint32_t a[4];
-      ldmatrix4_trans(vs + 16 * chunk_at(r, 2 * i + half), a);
+      ldmatrix4_trans(at + (i >> 2) * (KEYS * 128) + (x ^ ((2 * (i & 3)) << 4)), a);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -295,33 +305,30 @@ struct MmaTile {
 
 // Sums N values over the warp, each lane ending with the one of number lane_value<N>(lane): at every step a lane keeps half of its values and hands
 // over the rest, N - 1 + (5 - log2 N) shuffles in all instead of 5 N.
-template <int N> __device__ __forceinline__ float sum_exchange(float (&v)[N]) {
-  const int lane = threadIdx.x & 31;
-  int bit = 16;
+template <int N, int BIT = 16> __device__ __forceinline__ float sum_exchange(const float (&v)[N]) {
+  if constexpr (N > 1) {
+    const bool up = (threadIdx.x & BIT) != 0;
+    float half[N / 2];
 #pragma unroll
-  for (int n = N; n > 1; n >>= 1, bit >>= 1) {
-    const bool up = lane & bit;
+    for (int i = 0; i < N / 2; ++i) half[i] = (up ? v[i + N / 2] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + N / 2], BIT);
+    return sum_exchange<N / 2, BIT / 2>(half);
+  } else {
+    float x = v[0];
 #pragma unroll
-    for (int i = 0; i < n / 2; ++i) {
-      const float give = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
-    }
+    for (int b = BIT; b > 0; b >>= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
+    return x;
   }
-#pragma unroll
-  for (; bit > 0; bit >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);
-  return v[0];
 }
 // f32: a lane owns E neighbouring dimensions of all keys and rows; eight keys a tile.
-template <int DPAD_, int ROWS_, int STAGES_>
+template <int DPAD_, int ROWS_>
 struct F32Tile {
   using AT = float;
-  static constexpr int DPAD = DPAD_, ROWS = ROWS_, KEYS = 8, STAGES = STAGES_, CHUNKS = DPAD / 4, E = DPAD / 32;
+  static constexpr int DPAD = DPAD_, ROWS = ROWS_, KEYS = 8, E = DPAD / 32, CTAS = DPAD * ROWS > 512 ? 1 : 2;
   static constexpr bool kRedo = false;
   static constexpr int kSets = ROWS * KEYS > 32 ? ROWS * KEYS / 32 : 1, kN = ROWS * KEYS / kSets;  // kN values are summed at once
   static constexpr int kRowsOfSet = ROWS / kSets, kLog = kN == 32 ? 5 : kN == 16 ? 4 : 3;
   float q[ROWS][E], o[ROWS][E], m[ROWS], l[ROWS];  // m: the same in all lanes; l: a lane's own
   float slope[kSets];
-  static __device__ __forceinline__ int chunk_at(int r, int c) { return r * CHUNKS + c; }
 
   __device__ __forceinline__ void begin(const PagedArgs& p, int t, int kvh, int tile) {
     const int lane = threadIdx.x & 31;
@@ -343,13 +350,20 @@ struct F32Tile {
       slope[s] = p.slopes && row < p.rep ? p.slopes[kvh * p.rep + row] * kLog2e : 0.f;
     }
   }
-  static __device__ __forceinline__ void load(uint32_t at, float (&v)[E]) {
+  // this lane's dimensions of row r
+  static __device__ __forceinline__ void load(uint32_t tile_at, int r, float (&v)[E]) {
+    const int lane = threadIdx.x & 31;
     if (E == 2) {
+      const int c = lane >> 1;
+      const uint32_t at = tile_at + (c >> 3) * (KEYS * 128) + r * 128 + (((c & 7) ^ r) << 4) + 8 * (lane & 1);
       asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v[0]), "=f"(v[E - 1]) : "r"(at));
     } else {
 #pragma unroll
-      for (int e = 0; e + 3 < E; e += 4)
-        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[e]), "=f"(v[e + 1]), "=f"(v[e + 2]), "=f"(v[e + 3]) : "r"(at + 4 * e));
+      for (int e = 0; e + 3 < E; e += 4) {
+        const int c = (lane * E + e) >> 2;
+        const uint32_t at = tile_at + (c >> 3) * (KEYS * 128) + r * 128 + (((c & 7) ^ r) << 4);
+        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[e]), "=f"(v[e + 1]), "=f"(v[e + 2]), "=f"(v[e + 3]) : "r"(at));
+      }
     }
   }
   template <bool OPTIONS> __device__ __forceinline__ void take(const PagedArgs& p, uint32_t ks, uint32_t vs, uint32_t seen, int behind) {
@@ -358,7 +372,7 @@ struct F32Tile {
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
       float k[E];
-      load(ks + 4 * (j * DPAD + lane * E), k);
+      load(ks, j, k);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         float x = 0.f;
@@ -403,7 +417,7 @@ struct F32Tile {
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
       float v[E];
-      load(vs + 4 * (j * DPAD + lane * E), v);
+      load(vs, j, v);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         const float w = __shfl_sync(0xffffffffu, pr[r / kRowsOfSet], ((r % kRowsOfSet) * KEYS + j) << (5 - kLog));
@@ -425,9 +439,12 @@ struct F32Tile {
   }
 };
 
-// Dynamic shared memory: the warps' rings, then [4][rows] maxima, [4][rows] sums and [4][rows][DPAD + 4] outputs (the pitch keeps the lanes of a
-// quad in banks of their own), which join() uses too.
-template <class Tile> constexpr int kRingBytes = kWarps * Tile::STAGES * 2 * Tile::KEYS * Tile::DPAD * int(sizeof(typename Tile::AT));
+// A stage of the ring: a tile's keys, then its values, each in boxes of KEYS rows of 128 bytes (16-byte chunk c of row r at c ^ (r & 7)).
+template <class Tile> constexpr int kBoxBytes = Tile::KEYS * 128;
+template <class Tile> constexpr int kBoxes = Tile::DPAD * int(sizeof(typename Tile::AT)) / 128;
+template <class Tile> constexpr int kStageBytes = 2 * kBoxes<Tile> * kBoxBytes<Tile>;
+// Behind the ring: [4][rows] maxima, [4][rows] sums and [4][rows][DPAD + 4] outputs of the consumer warps (the pitch keeps the lanes of a quad in
+// banks of their own), which join() uses too.
 template <class Tile> constexpr int kPitch = Tile::DPAD + 4;
 template <class Tile> constexpr int area_bytes(int rows) { return kWarps * rows * (2 + kPitch<Tile>) * int(sizeof(float)); }
 // A part in scratch: [ROWS][DPAD] outputs, then [ROWS] maxima and [ROWS] sums; whole 16-byte vectors
@@ -438,7 +455,7 @@ template <class Tile> constexpr int kSlotSum = kSlotMax<Tile> + Tile::ROWS;
 // The slot in which CTA first + i of a token's CTAs leaves its part: the first of them starts the token, the others have it begun elsewhere.
 __device__ __forceinline__ int slot_of(int first, int i) { return 2 * (first + i) + (i == 0 ? 1 : 0); }
 // Parts i = from, from + step, ... of a token, `count` of them (at most 32), become one in area: [rows][DPAD] outputs, [rows] maxima, [rows] sums, and
-// then the [rows][count] factors used.
+// then the [rows][count] factors used.  The consumer warps call it.
 template <class Tile> __device__ void join(const float* slots, int first, int from, int step, int count, int rows, float* area) {
   float *maxima = area + rows * Tile::DPAD, *sums = maxima + rows, *factor = sums + rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -456,8 +473,8 @@ template <class Tile> __device__ void join(const float* slots, int first, int fr
     if (lane < count) factor[r * count + lane] = f;
     if (lane == 0) { maxima[r] = top; sums[r] = sum; }
   }
-  __syncthreads();
-  for (int e = threadIdx.x * 4; e < rows * Tile::DPAD; e += kThreads * 4) {
+  consumers_meet();
+  for (int e = threadIdx.x * 4; e < rows * Tile::DPAD; e += kConsumers * 4) {
     const int r = e / Tile::DPAD;
     const float* at = slots + e;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -469,41 +486,46 @@ template <class Tile> __device__ void join(const float* slots, int first, int fr
     }
     *reinterpret_cast<float4*>(area + e) = a;
   }
-  __syncthreads();
+  consumers_meet();
 }
 
-template <class Tile, bool OPTIONS>
-__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedArgs p) {
+template <class Tile, bool OPTIONS, bool TMA>
+__global__ void __launch_bounds__(kThreads, Tile::CTAS)
+    paged_attention_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using AT = typename Tile::AT;
-  constexpr int DPAD = Tile::DPAD, KEYS = Tile::KEYS, STAGES = Tile::STAGES, UNIT = KEYS * kWarps, CHUNKS = Tile::CHUNKS;
-  constexpr int kTileBytes = KEYS * DPAD * int(sizeof(AT)), kCopies = KEYS * CHUNKS / 32, kPerChunk = 16 / int(sizeof(AT));
-  extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ long long found_begin, scan[kWarps];
-  __shared__ int found_token, is_last;
-  __shared__ uint32_t seen_of[kWarps][STAGES];
+  constexpr int DPAD = Tile::DPAD, KEYS = Tile::KEYS, kHalf = kStageBytes<Tile> / 2, kPerChunk = 16 / int(sizeof(AT));
+  constexpr uint32_t kAll = (1u << KEYS) - 1;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
+  __shared__ uint32_t seen_of[kMaxStages];
+  __shared__ long long found_begin, scan[kThreads / 32];
+  __shared__ int found_token, is_last, abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = int(blockIdx.x);
-  float* area = reinterpret_cast<float*>(sm + kRingBytes<Tile>);
-  const uint32_t ring = smem_at(sm) + warp * STAGES * 2 * kTileBytes;
-  if (p.head_dim < DPAD) {  // the copies leave the padding alone: it is zero from here on
-    for (int i = threadIdx.x; i < kRingBytes<Tile> / 16; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], TMA ? 1 : 33);  // cp.async: every lane's copies, and the word of what is seen
+      mbar_init(&empty[s], 1);
+    }
+    abort_flag = 0;
+    mbar_fence_init();
+    if (TMA) { tma_prefetch_desc(&k_map); tma_prefetch_desc(&v_map); }
+  }
+  if (p.head_dim < DPAD) {  // no copy writes the padding: it is zero from here on
+    for (int i = threadIdx.x; i < p.stages * (kStageBytes<Tile> / 16); i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   tl_pdl_wait();
 
-  // Tokens that see nothing, and how many units the others have
+  // Tokens that see nothing, and how many tiles the others have
   const int segs = p.n_kv_heads * p.row_tiles, chunk = (p.tokens + kThreads - 1) / kThreads;
   const int t_first = min(p.tokens, int(threadIdx.x) * chunk), t_end = min(p.tokens, t_first + chunk);
+  auto tiles_of = [&](const Token& k) { return tl_units(k.lo / KEYS * KEYS, k.hi, KEYS); };
   long long mine = 0;
-  for (int t = t_first; t < t_end; ++t) {
-    const Token k = token_of(p, t, t % int(gridDim.x) == cta);
-    mine += tl_units(k.lo, k.hi, UNIT);
-  }
-  for (int t = cta; t < p.tokens; t += int(gridDim.x)) {
-    const Token k = token_of(p, t, false);
-    if (k.hi == 0)
+  for (int t = t_first; t < t_end; ++t) mine += tiles_of(token_of(p, t, t % int(gridDim.x) == cta));
+  for (int t = cta; t < p.tokens; t += int(gridDim.x))
+    if (token_of(p, t, false).hi == 0)
       for (int e = threadIdx.x; e < p.n_heads * p.head_dim; e += kThreads)
         reinterpret_cast<AT*>(p.out)[int64_t(t) * p.n_heads * p.head_dim + e] = DT<AT>::from_f32(0.f);
-  }
   long long to = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -514,7 +536,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   __syncthreads();
   long long whole = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) to += scan[w];
     whole += scan[w];
   }
@@ -525,8 +547,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   if ((to - mine) * segs <= begin && begin < to * segs) {  // one thread's
     long long at = (to - mine) * segs;
     for (int t = t_first; t < t_end; ++t) {
-      const Token k = token_of(p, t, false);
-      const long long n = (long long)(tl_units(k.lo, k.hi, UNIT)) * segs;
+      const long long n = (long long)(tiles_of(token_of(p, t, false))) * segs;
       if (begin < at + n) {
         found_token = t;
         found_begin = begin - at;
@@ -536,90 +557,143 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     }
   }
   __syncthreads();
-
   Cursor c;
   c.t = found_token;
-  c.template open<UNIT>(p);
+  c.template open<KEYS>(p);
   c.seg = int(found_begin / c.n);
   c.u = int(found_begin - (long long)(c.seg) * c.n);
   c.head(p);
-  Cursor f = c;  // what is fetched next
 
-  // A lane below KEYS finds its key's row a unit before it is copied: the table is read on the way
-  bool row_seen;
-  int64_t row_at;
-  auto look_up = [&](bool more) {
-    const int key = f.k.lo + f.u * UNIT + warp * KEYS + lane;
-    row_seen = more && lane < KEYS && key < f.k.hi;
-    row_at = 0;
-    if (row_seen) {
-      const int index = tl_divide(key, p.page_div), page = __ldg(p.page_table + f.k.seq * p.max_pages + index);
-      if (tl_bad_page(page, p.n_pages)) {
-        atomicOr(p.status, kBadPage);
-        row_seen = false;
-      } else {
-        row_at = tl_page_at(page, key - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim) + int64_t(f.kvh) * p.page_size * p.head_dim;
-      }
-    }
-  };
-  auto fetch = [&](int stage) {
-    const uint32_t seen = __ballot_sync(0xffffffffu, row_seen);
-    if (lane == 0) seen_of[warp][stage] = seen;
-    const uint32_t ks = ring + stage * 2 * kTileBytes, vs = ks + kTileBytes;
-    if (seen) {
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const int e = i * 32 + lane, r = e / CHUNKS, ch = e % CHUNKS;
-        const int64_t at = __shfl_sync(0xffffffffu, row_at, r) + ch * kPerChunk;
-        const int bytes = (seen >> r) & 1 ? 16 : 0;
-        if (ch * kPerChunk < p.head_dim) {
-          copy16(ks + 16 * Tile::chunk_at(r, ch), reinterpret_cast<const AT*>(p.k_pages) + at, bytes);
-          copy16(vs + 16 * Tile::chunk_at(r, ch), reinterpret_cast<const AT*>(p.v_pages) + at, bytes);
+  if (warp == kWarps) {
+    // ---- the producer.  A lane looks up a tile's page (cp.async: a row's) a batch before it is copied, so that the table is read on the way.
+    constexpr int kBatch = TMA ? 32 : 1;
+    struct Batch {
+      int n, key0, kvh, key, page;  // n tiles from key0 on; this lane's key and its page
+      Token k;
+    };
+    long long left = end - begin;
+    auto look_up = [&]() {
+      Batch b;
+      b.n = int(min((long long)(min(kBatch, c.n - c.u)), left));
+      b.k = c.k;
+      b.kvh = c.kvh;
+      b.key0 = c.template first_key<KEYS>(c.u);
+      b.key = b.key0 + (TMA ? lane * KEYS : lane);
+      b.page = -1;
+      if (TMA ? lane < b.n : lane < KEYS && b.key >= b.k.lo && b.key < b.k.hi) b.page = __ldg(p.page_table + b.k.seq * p.max_pages + tl_divide(b.key, p.page_div));
+      left -= b.n;
+      c.u += b.n;
+      if (c.u == c.n && left > 0) c.template next<KEYS>(p);
+      return b;
+    };
+    Batch now = look_up();
+    int stage = 0, issued = 0;
+    uint32_t parity = 1;  // of the phase before the first: the ring is empty
+    bool ok = true;
+    while (now.n > 0 && ok) {
+      Batch then;
+      then.n = 0;
+      if (left > 0) then = look_up();
+      const bool wanted = TMA ? lane < now.n : lane < KEYS && now.key >= now.k.lo && now.key < now.k.hi, there = wanted && !tl_bad_page(now.page, p.n_pages);
+      if (wanted && !there) atomicOr(p.status, kBadPage);
+      const int in_page = now.key - tl_divide(now.key, p.page_div) * p.page_size;
+      const int64_t row = (int64_t(now.page) * p.n_kv_heads + now.kvh) * p.page_size + in_page;
+      for (int j = 0; j < now.n; ++j) {
+        if (!mbar_wait_all(&empty[stage], parity, &abort_flag)) { ok = false; break; }
+        uint8_t* at = sm + stage * kStageBytes<Tile>;
+        if (TMA) {
+          const int key0 = now.key0 + j * KEYS, y = __shfl_sync(0xffffffffu, int(row), j);
+          const bool copied = __shfl_sync(0xffffffffu, int(there), j) != 0;
+          if (lane == 0) {
+            uint32_t seen = kAll;
+            if (key0 < now.k.lo) seen &= kAll << (now.k.lo - key0);
+            if (key0 + KEYS > now.k.hi) seen &= kAll >> (key0 + KEYS - now.k.hi);
+            seen_of[stage] = copied ? seen : 0;
+            if (copied) {
+              const int boxes = (p.head_dim * int(sizeof(AT)) + 127) / 128;
+              mbar_expect_tx(&full[stage], uint32_t(2 * boxes * kBoxBytes<Tile>));
+              for (int b = 0; b < boxes; ++b) {
+                tma_load_2d(at + b * kBoxBytes<Tile>, &k_map, b * (128 / int(sizeof(AT))), y, &full[stage]);
+                tma_load_2d(at + kHalf + b * kBoxBytes<Tile>, &v_map, b * (128 / int(sizeof(AT))), y, &full[stage]);
+              }
+            } else {
+              mbar_arrive(&full[stage]);
+            }
+          }
+          ++issued;
+        } else {
+          const uint32_t seen = __ballot_sync(0xffffffffu, there);
+          const uint32_t ks = smem_u32(at), vs = ks + kHalf;
+          const int chunks = p.head_dim / kPerChunk;
+          for (int r = 0; r < KEYS; ++r) {
+            const int64_t from = __shfl_sync(0xffffffffu, row, r) * p.head_dim;
+            const int bytes = (seen >> r) & 1 ? 16 : 0;
+            for (int ch = lane; ch < chunks; ch += 32) {
+              const uint32_t to_at = (ch >> 3) * kBoxBytes<Tile> + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+              const int64_t e = bytes ? from + ch * kPerChunk : 0;
+              copy16(ks + to_at, reinterpret_cast<const AT*>(p.k_pages) + e, bytes);
+              copy16(vs + to_at, reinterpret_cast<const AT*>(p.v_pages) + e, bytes);
+            }
+          }
+          copy_arrive(&full[stage]);
+          if (lane == 0) {
+            seen_of[stage] = seen;
+            mbar_arrive(&full[stage]);
+          }
         }
+        if (++stage == p.stages) { stage = 0; parity ^= 1; }
       }
+      now = then;
     }
-    copy_commit();
-  };
-  long long ahead = begin;  // units fetched
-  look_up(true);
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    if (ahead < end) {
-      fetch(s);
-      if (++ahead < end) { f.template next<UNIT>(p); look_up(true); }
-    } else {
-      copy_commit();
+    if (!ok) {
+      if (lane == 0) { atomicExch(&abort_flag, 1); atomicExch(p.wait_status, TL_DEV_TIMEOUT_EMPTY); }
+      if (TMA && lane == 0) tma_drain(full, p.stages, issued);
+      if (!TMA) asm volatile("cp.async.wait_all;" ::: "memory");
     }
+    return;
   }
 
+  // ---- the consumers: warp w takes the share's tiles w, w + 4, ...
+  float* area = reinterpret_cast<float*>(sm + p.stages * kStageBytes<Tile>);
+  int stage = warp, parity = 0;
+  while (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
+  bool ok = true;
+  long long next = begin + warp, at = begin;  // this warp's next tile; the first of the current token's and group's in the share
   Tile tile;
-  tile.begin(p, c.t, c.kvh, c.tile);
-  int stage = 0;
-  for (long long w = begin; w < end; ++w) {
-    copy_wait<STAGES - 2>();
-    __syncwarp();  // this unit's rows have landed for all lanes, and all have read the last one's
-    const uint32_t seen = seen_of[warp][stage];
-    {
-      const int to_fill = stage == 0 ? STAGES - 1 : stage - 1;
-      if (ahead < end) {
-        fetch(to_fill);
-        if (++ahead < end) { f.template next<UNIT>(p); look_up(true); }
-      } else {
-        copy_commit();
+  while (at < end) {
+    tile.begin(p, c.t, c.kvh, c.tile);
+    const long long seg_begin = at - c.u, seg_end = seg_begin + c.n, stop = min(seg_end, end);
+    for (; next < stop; next += kWarps) {
+      if (ok && !mbar_wait_all(&full[stage], parity, &abort_flag)) {
+        ok = false;
+        if (lane == 0) { atomicExch(&abort_flag, 1); atomicExch(p.wait_status, TL_DEV_TIMEOUT_FULL); }
       }
+      if (ok) {
+        const uint32_t seen = seen_of[stage], ks = smem_u32(sm + stage * kStageBytes<Tile>);
+        if (seen) {
+          if (TMA && seen != kAll) {  // values that do not count, whatever they are
+            for (int i = lane; i < KEYS * kBoxes<Tile> * 8; i += 32) {
+              const int r = (i >> 3) % KEYS;
+              if (!((seen >> r) & 1)) reinterpret_cast<uint4*>(sm + stage * kStageBytes<Tile> + kHalf)[i] = make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
+          }
+          tile.template take<OPTIONS>(p, ks, ks + kHalf, seen, c.template first_key<KEYS>(int(next - seg_begin)) + 1 - c.k.hi);
+          if (TMA && seen != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+      }
+      stage += kWarps;
+      while (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
     }
-    const uint32_t ks = ring + stage * 2 * kTileBytes;
-    if (seen) tile.template take<OPTIONS>(p, ks, ks + kTileBytes, seen, c.k.lo + c.u * UNIT + warp * KEYS + 1 - c.k.hi);
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-    if (c.u + 1 < c.n && w + 1 < end) { ++c.u; continue; }
 
-    // The last unit of this token and group, or of this CTA's share
+    // The last tile of this token and group, or of this CTA's share
     const int rows = min(Tile::ROWS, p.rep - c.tile * Tile::ROWS), h0 = c.kvh * p.rep + c.tile * Tile::ROWS;
     float *wm = area, *wl = wm + kWarps * rows, *wo = wl + kWarps * rows;
-    const long long seg_begin = w - c.u, seg_end = seg_begin + c.n;
     const bool starts = seg_begin >= begin, ends = seg_end <= end;
     tile.end(wm + warp * rows, wl + warp * rows, wo + warp * rows * kPitch<Tile>, kPitch<Tile>, rows);
-    __syncthreads();
+    consumers_meet();
     auto store = [&](int r, int d, float v) {  // a warp's 32 values are one row's
       if (Tile::kRedo && __any_sync(0xffffffffu, d < p.head_dim && !isfinite(v))) {
         row_again<AT>(p, c.k, c.k.hi - 1, c.t, h0 + r, c.kvh, d & ~31);
@@ -628,7 +702,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       }
     };
     float* slot = p.slots + int64_t(2 * cta + (starts ? 1 : 0)) * slot_floats<Tile>();
-    for (int e = threadIdx.x; e < rows * DPAD; e += kThreads) {
+    for (int e = threadIdx.x; e < rows * DPAD; e += kConsumers) {
       const int r = e / DPAD, d = e - r * DPAD;
       float top = -INFINITY;
 #pragma unroll
@@ -654,12 +728,12 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       const int group = (cta - first) / kGroup, groups = (count + kGroup - 1) / kGroup, members = min(kGroup, count - group * kGroup);
       auto last_of = [&](unsigned* arrived, int of) {
         __threadfence();
-        __syncthreads();
+        consumers_meet();
         if (threadIdx.x == 0) {
           is_last = atomicAdd(arrived, 1u) == unsigned(of) - 1;
           if (is_last) *arrived = 0;  // for the next launch
         }
-        __syncthreads();
+        consumers_meet();
         __threadfence();
         return is_last != 0;
       };
@@ -668,7 +742,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         join<Tile>(p.slots, first, group * kGroup, 1, members, rows, area);
         if (groups > 1) {
           float* to_slot = p.slots + int64_t(slot_of(first, group * kGroup)) * slot_floats<Tile>();
-          for (int e = threadIdx.x; e < rows * DPAD; e += kThreads) __stcg(to_slot + e, area[e]);
+          for (int e = threadIdx.x; e < rows * DPAD; e += kConsumers) __stcg(to_slot + e, area[e]);
           if (int(threadIdx.x) < rows) {
             __stcg(to_slot + kSlotMax<Tile> + threadIdx.x, area[rows * DPAD + threadIdx.x]);
             __stcg(to_slot + kSlotSum<Tile> + threadIdx.x, area[rows * DPAD + rows + threadIdx.x]);
@@ -678,64 +752,74 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         }
       }
       if (done)
-        for (int e = threadIdx.x; e < rows * DPAD; e += kThreads) {
+        for (int e = threadIdx.x; e < rows * DPAD; e += kConsumers) {
           const int r = e / DPAD;
           const float sum = area[rows * DPAD + rows + r];
           store(r, e - r * DPAD, sum == 0.f ? 0.f : area[e] / sum);
         }
     }
-    __syncthreads();
-    if (w + 1 < end) {
-      c.template next<UNIT>(p);
-      tile.begin(p, c.t, c.kvh, c.tile);
+    at = stop;
+    if (at < end) {
+      c.template next<KEYS>(p);
+      consumers_meet();  // the area is free again
     }
   }
 }
 
-// CTAs that are resident together: by shared memory, two where the ring allows
-template <class Tile> int resident(int rows) { return std::min(2, 233472 / (kRingBytes<Tile> + area_bytes<Tile>(rows) + 1024 + 512)); }
-
-template <class Tile, bool OPTIONS> cudaError_t launch(tl_ctx* ctx, const PagedArgs& p, int64_t most_units) {
-  const int rows = std::min(Tile::ROWS, p.rep), smem = kRingBytes<Tile> + area_bytes<Tile>(rows);
-  auto kernel = paged_attention_kernel<Tile, OPTIONS>;
+template <class Tile, bool OPTIONS, bool TMA>
+cudaError_t launch(tl_ctx* ctx, PagedArgs& p, const CUtensorMap& k_map, const CUtensorMap& v_map, int64_t most_units) {
+  // Shared memory in equal parts for the resident CTAs (1 KB of each is the system's, the barriers take less than another)
+  const int rows = std::min(Tile::ROWS, p.rep), room = (228 / Tile::CTAS - 2) * 1024 - area_bytes<Tile>(rows);
+  p.stages = std::min(kMaxStages, room / kStageBytes<Tile>);
+  const int smem = p.stages * kStageBytes<Tile> + area_bytes<Tile>(rows);
+  auto kernel = paged_attention_kernel<Tile, OPTIONS, TMA>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>(int64_t(ctx->sm_count) * resident<Tile>(rows), std::max<int64_t>(1, most_units))));
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(int64_t(ctx->sm_count) * Tile::CTAS, std::max<int64_t>(1, most_units))));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[1] = {tl_pdl_attribute()};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p, k_map, v_map);
 }
 template <class Tile> cudaError_t launch_tile(tl_ctx* ctx, PagedArgs& p, int64_t longest) {
+  using AT = typename Tile::AT;
   p.row_tiles = (p.rep + Tile::ROWS - 1) / Tile::ROWS;
-  constexpr int kUnit = Tile::KEYS * kWarps;
-  const int64_t most = int64_t(p.tokens) * p.n_kv_heads * p.row_tiles * ((longest + kUnit - 1) / kUnit);
-  return p.softcap > 0.f || p.slopes ? launch<Tile, true>(ctx, p, most) : launch<Tile, false>(ctx, p, most);
+  const int64_t most = int64_t(p.tokens) * p.n_kv_heads * p.row_tiles * (longest / Tile::KEYS + 2);
+  // TMA boxes are whole 128-byte columns of a tile's rows, which are neighbours where a page holds whole tiles; their coordinates are int32
+  const int64_t all_rows = p.n_pages * p.n_kv_heads * p.page_size;
+  CUtensorMap k_map{}, v_map{};
+  constexpr int kColumns = 128 / int(sizeof(AT));
+  const bool tma = p.page_size % Tile::KEYS == 0 && p.head_dim >= kColumns && all_rows > 0 && all_rows <= INT32_MAX &&
+                   tl_encode_tmap_2d(&k_map, int(sizeof(AT)), p.k_pages, uint64_t(p.head_dim), uint64_t(all_rows), uint64_t(p.head_dim) * sizeof(AT), kColumns,
+                                     Tile::KEYS, 3) &&
+                   tl_encode_tmap_2d(&v_map, int(sizeof(AT)), p.v_pages, uint64_t(p.head_dim), uint64_t(all_rows), uint64_t(p.head_dim) * sizeof(AT), kColumns,
+                                     Tile::KEYS, 3);
+  const bool options = p.softcap > 0.f || p.slopes;
+  if (tma) return options ? launch<Tile, true, true>(ctx, p, k_map, v_map, most) : launch<Tile, false, true>(ctx, p, k_map, v_map, most);
+  return options ? launch<Tile, true, false>(ctx, p, k_map, v_map, most) : launch<Tile, false, false>(ctx, p, k_map, v_map, most);
 }
 // Up to 8 query heads of a KV head on one tile, up to 16 on a tile of two, more on several; 256 dimensions leave registers for 8 (f32: 4).
 template <typename AT> cudaError_t launch_mma(tl_ctx* ctx, PagedArgs& p, int64_t longest) {
-  if (p.head_dim <= 64) return p.rep <= 8 ? launch_tile<MmaTile<AT, 64, 1, 4>>(ctx, p, longest) : launch_tile<MmaTile<AT, 64, 2, 4>>(ctx, p, longest);
-  if (p.head_dim <= 128) return p.rep <= 8 ? launch_tile<MmaTile<AT, 128, 1, 3>>(ctx, p, longest) : launch_tile<MmaTile<AT, 128, 2, 3>>(ctx, p, longest);
-  return launch_tile<MmaTile<AT, 256, 1, 3>>(ctx, p, longest);
+  if (p.head_dim <= 64) return p.rep <= 8 ? launch_tile<MmaTile<AT, 64, 1>>(ctx, p, longest) : launch_tile<MmaTile<AT, 64, 2>>(ctx, p, longest);
+  if (p.head_dim <= 128) return p.rep <= 8 ? launch_tile<MmaTile<AT, 128, 1>>(ctx, p, longest) : launch_tile<MmaTile<AT, 128, 2>>(ctx, p, longest);
+  return launch_tile<MmaTile<AT, 256, 1>>(ctx, p, longest);
 }
 cudaError_t launch_f32(tl_ctx* ctx, PagedArgs& p, int64_t longest) {
   if (p.head_dim <= 64)
-    return p.rep == 1 ? launch_tile<F32Tile<64, 1, 4>>(ctx, p, longest) : p.rep <= 4 ? launch_tile<F32Tile<64, 4, 4>>(ctx, p, longest) : launch_tile<F32Tile<64, 8, 4>>(ctx, p, longest);
+    return p.rep == 1 ? launch_tile<F32Tile<64, 1>>(ctx, p, longest) : p.rep <= 4 ? launch_tile<F32Tile<64, 4>>(ctx, p, longest) : launch_tile<F32Tile<64, 8>>(ctx, p, longest);
   if (p.head_dim <= 128)
-    return p.rep == 1 ? launch_tile<F32Tile<128, 1, 3>>(ctx, p, longest) : p.rep <= 4 ? launch_tile<F32Tile<128, 4, 3>>(ctx, p, longest) : launch_tile<F32Tile<128, 8, 3>>(ctx, p, longest);
-  return p.rep == 1 ? launch_tile<F32Tile<256, 1, 3>>(ctx, p, longest) : launch_tile<F32Tile<256, 4, 3>>(ctx, p, longest);
+    return p.rep == 1 ? launch_tile<F32Tile<128, 1>>(ctx, p, longest) : p.rep <= 4 ? launch_tile<F32Tile<128, 4>>(ctx, p, longest) : launch_tile<F32Tile<128, 8>>(ctx, p, longest);
+  return p.rep == 1 ? launch_tile<F32Tile<256, 1>>(ctx, p, longest) : launch_tile<F32Tile<256, 4>>(ctx, p, longest);
 }
 
 // Parts of tokens for two CTAs an SM of the largest slot, and the arrivals: one size for all calls, so that no captured call's scratch is replaced.
-constexpr int kSlotFloats = 16 * 130, kLeastUnits = 4;
-static_assert(slot_floats<MmaTile<__half, 64, 2, 4>>() <= kSlotFloats && slot_floats<F32Tile<256, 4, 3>>() <= kSlotFloats && slot_floats<F32Tile<128, 8, 3>>() <= kSlotFloats, "slots");
-static_assert(slot_floats<MmaTile<__half, 256, 1, 3>>() <= kSlotFloats && slot_floats<MmaTile<__half, 128, 2, 3>>() <= kSlotFloats, "slots");
+constexpr int kSlotFloats = 16 * 130, kLeastUnits = 16;
+static_assert(slot_floats<MmaTile<__half, 64, 2>>() <= kSlotFloats && slot_floats<F32Tile<256, 4>>() <= kSlotFloats && slot_floats<F32Tile<128, 8>>() <= kSlotFloats, "slots");
+static_assert(slot_floats<MmaTile<__half, 256, 1>>() <= kSlotFloats && slot_floats<MmaTile<__half, 128, 2>>() <= kSlotFloats, "slots");
 int32_t secure_scratch(tl_ctx* ctx) {
   if (ctx->paged_scratch) return TL_OK;
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
@@ -789,6 +873,7 @@ int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32
   p.window = window; p.scale = scale; p.softcap = softcap; p.least_units = kLeastUnits;
   p.page_div = tl_divide_by(cache->page_size);
   p.status = ctx->dev_status + 1;
+  p.wait_status = ctx->dev_status;
   p.slots = reinterpret_cast<float*>(ctx->paged_scratch);
   p.arrivals = reinterpret_cast<unsigned*>(p.slots + size_t(ctx->sm_count) * 2 * 2 * kSlotFloats);
   int64_t longest = int64_t(cache->max_pages) * cache->page_size;

@@ -68,6 +68,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
+// The same by a whole warp: all of its lanes, or none
+__device__ __forceinline__ bool mbar_wait_all(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
 // A wait that the abort flag does not end, still bounded.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
   for (int it = 0; it < kWaitTimeoutIters && !mbar_try_wait(bar, parity); ++it) {}
