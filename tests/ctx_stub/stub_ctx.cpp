@@ -14,10 +14,11 @@ extern "C" int stub_bad_token(int pos, long long seq, int n_seqs, int max_pages,
 }
 extern "C" int stub_bad_page(int page, long long n_pages) { return tl_bad_page(page, n_pages); }
 extern "C" long long stub_page_at(int page, int slot, int heads, int page_size, int dim) { return tl_page_at(page, slot, heads, page_size, dim); }
-extern "C" int stub_units(int first, int end, int keys) { return tl_units(first, end, keys); }
-extern "C" long long stub_share_begin(long long units, int ctas, int cta) { return tl_share_begin(units, ctas, cta); }
-extern "C" int stub_share_owner(long long units, int ctas, long long unit) { return tl_share_owner(units, ctas, unit); }
-extern "C" int stub_share_ctas(long long units, int most, int least) { return tl_share_ctas(units, most, least); }
+extern "C" int stub_lead() { return kLead; }
+extern "C" int stub_tiles(int first, int end, int keys) { return tl_tiles(first, end, keys); }
+extern "C" int stub_share_ctas(long long units, int most, int least, long long parts) { return tl_shares(units, most, least, parts).ctas; }
+extern "C" long long stub_share_begin(long long units, int most, int least, long long parts, int cta) { return tl_share_begin(tl_shares(units, most, least, parts), cta); }
+extern "C" int stub_share_owner(long long units, int most, int least, long long parts, long long unit) { return tl_share_owner(tl_shares(units, most, least, parts), unit); }
 // The first n at which the quotient by d is wrong, of `count` neighbours of every multiple that is tried; -1: none
 extern "C" long long stub_divide_wrong(int d, int tries) {
   const TlDivide by = tl_divide_by(d);

@@ -25,8 +25,9 @@ def stub(tmp_path_factory):
     lib.stub_bad_page.argtypes = [C.c_int, C.c_longlong]
     lib.stub_page_at.argtypes = [C.c_int] * 5
     lib.stub_page_at.restype = C.c_longlong
-    for name, kinds, result in (("share_begin", [C.c_longlong, C.c_int, C.c_int], C.c_longlong), ("share_owner", [C.c_longlong, C.c_int, C.c_longlong], C.c_int),
-                                ("share_ctas", [C.c_longlong, C.c_int, C.c_int], C.c_int), ("divide_wrong", [C.c_int, C.c_int], C.c_longlong)):
+    shares = [C.c_longlong, C.c_int, C.c_int, C.c_longlong]
+    for name, kinds, result in (("share_ctas", shares, C.c_int), ("share_begin", shares + [C.c_int], C.c_longlong), ("share_owner", shares + [C.c_longlong], C.c_int),
+                                ("divide_wrong", [C.c_int, C.c_int], C.c_longlong)):
         f = getattr(lib, "stub_" + name)
         f.argtypes, f.restype = kinds, result
     return lib
@@ -152,42 +153,56 @@ def test_only_indexes_in_range_become_addresses(stub):
 
 
 def test_every_unit_has_one_owner(stub):
-    """The shares cover the units without gaps, none is empty, and the owner of a unit is the CTA whose share holds it."""
-    for units, most, least in itertools.product([1, 2, 3, 4, 5, 37, 295, 296, 297, 1000, 40_001], [1, 2, 148, 296], [1, 4]):
-        ctas = stub.stub_share_ctas(units, most, least)
-        assert 1 <= ctas <= most and (ctas == most or ctas * least >= units) and ctas <= units
-        begins = [stub.stub_share_begin(units, ctas, c) for c in range(ctas + 1)]
-        assert begins[0] == 0 and begins[-1] == units and all(a < b for a, b in zip(begins, begins[1:]))
+    """The shares cover the units without gaps, each is long enough to hold a tile, and the owner of a unit is the CTA whose share holds it."""
+    lead = stub.stub_lead()
+    for units, most, least, parts in itertools.product([lead + 1, lead + 2, 37, 295, 296, 297, 1000, 40_001], [1, 2, 148, 296], [1, 24], [1, 8, 300, 5000]):
+        args = units, most, least, parts
+        ctas = stub.stub_share_ctas(*args)
+        assert 1 <= ctas <= most and ctas * (lead + 1) <= units and (ctas >= min(units // least, most) or ctas == units // (lead + 1))
+        begins = [stub.stub_share_begin(*args, c) for c in range(ctas + 1)]
+        assert begins[0] == 0 and begins[-1] == units and all(b - a >= lead + 1 for a, b in zip(begins, begins[1:]))
+        assert max(b - a for a, b in zip(begins, begins[1:])) - min(b - a for a, b in zip(begins, begins[1:])) <= 1
         for c in range(ctas):
-            assert stub.stub_share_owner(units, ctas, begins[c]) == c and stub.stub_share_owner(units, ctas, begins[c + 1] - 1) == c
-    big = (1 << 40) + 12345  # units of a call at the limits
+            assert stub.stub_share_owner(*args, begins[c]) == c and stub.stub_share_owner(*args, begins[c + 1] - 1) == c
+    big = (1 << 40) + 12345, 296, 24, 1  # units of a call at the limits
     for c in range(296):
-        assert stub.stub_share_owner(big, 296, stub.stub_share_begin(big, 296, c)) == c
-    assert [stub.stub_units(a, b, 64) for a, b in ((0, 0), (5, 5), (0, 1), (0, 64), (0, 65), (3, 67), (2 ** 31 - 66, 2 ** 31 - 1))] == [0, 0, 1, 1, 2, 1, 2]
+        assert stub.stub_share_owner(*big, stub.stub_share_begin(*big, c)) == c == stub.stub_share_owner(*big, stub.stub_share_begin(*big, c + 1) - 1)
+    assert [stub.stub_tiles(a, b, 16) for a, b in ((0, 0), (5, 5), (0, 1), (0, 16), (0, 17), (3, 19), (15, 17), (16, 17), (2 ** 31 - 20, 2 ** 31 - 17), (2 ** 31 - 20, 2 ** 31 - 1))] == [
+        0, 0, 1, 1, 2, 2, 2, 1, 1, 2]
 
 
-def test_parts_of_a_token_meet_in_slots_of_their_own(stub):
-    """Walked on the host: each CTA leaves at most one part in each of its two slots, the CTAs between a token's first and last owner are those that leave one, and
-    no two tokens' groups of sixteen count their arrivals in the same place."""
-    for lengths, ctas in (([1, 7, 300, 2, 2, 90], 37), ([5000], 296), ([33] * 50, 296), ([1000, 1, 1, 999], 296)):
-        units = sum(lengths)
-        parts, places, at = {}, set(), 0
-        for n in lengths:
-            first, last = (stub.stub_share_owner(units, ctas, u) for u in (at, at + n - 1))
-            for c in range(first, last + 1):
-                begin, end = (stub.stub_share_begin(units, ctas, x) for x in (c, c + 1))
-                assert begin < at + n and end > at  # it has some of the token
-                starts = at >= begin
-                assert starts == (c == first)
-                if first != last:
-                    slot = 2 * c + starts
-                    assert slot not in parts
-                    parts[slot] = at
-                    if (c - first) % 16 == 0:
-                        place = 2 * c + (c == first)
-                        assert place not in places and place < 2 * ctas
-                        places.add(place)
-            at += n
+@pytest.mark.parametrize("tiles,most", [([1, 7, 300, 2, 2, 90], 37), ([5000], 296), ([33] * 50, 296), ([1000, 1, 1, 999], 296), ([1] * 700, 296), ([3, 1] * 20, 148),
+                                        ([1], 296), ([1, 1], 296), ([2000] + [1] * 100, 148)])
+def test_parts_meet_in_slots_of_their_own(stub, tiles, most):
+    """The shares walked on the host as the kernel walks them: every tile is taken once, the CTAs that have tiles of a part are those between the owners of its first and
+    last, each leaves what it made of a part in a slot that no other part uses, and no two groups of sixteen count their arrivals in one place."""
+    lead = stub.stub_lead()
+    starts_at = list(itertools.accumulate([0] + [lead + n for n in tiles]))
+    args = starts_at[-1], most, 24, len(tiles)
+    ctas, taken, slots, places = stub.stub_share_ctas(*args), [0] * len(tiles), set(), set()
+    for cta in range(ctas):
+        begin, end = (stub.stub_share_begin(*args, x) for x in (cta, cta + 1))
+        has = 0
+        for part, n in enumerate(tiles):
+            tile0 = starts_at[part] + lead
+            u, stop = max(0, begin - tile0), min(n, end - tile0)
+            if u >= stop:
+                continue
+            has += stop - u
+            assert taken[part] == u
+            taken[part] = stop
+            first, last = (stub.stub_share_owner(*args, x) for x in (tile0, tile0 + n - 1))
+            assert first <= cta <= last and (cta == first) == (u == 0) and (cta == last) == (stop == n)
+            if (u, stop) != (0, n):
+                slot = 2 * cta + (u == 0)
+                assert slot not in slots
+                slots.add(slot)
+                if (cta - first) % 16 == 0:
+                    place = 2 * cta + (cta == first)
+                    assert place not in places and place < 2 * most
+                    places.add(place)
+        assert has > 0
+    assert taken == tiles
 
 
 @pytest.mark.parametrize("d", [1, 2, 3, 5, 7, 16, 24, 48, 100, 255, 256, 257, 641, 65_535, 65_537, 1_000_003, 2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1])

@@ -105,9 +105,9 @@ int32_t tl_check_paged(tl_ctx* ctx, const char* who, const tl_paged_cache* c, co
   if (!positions || !c->k_pages || !c->v_pages || !c->page_table) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "%s: null pointer", who);
   if (!token_seq && tokens > c->n_seqs)
     return tl_set_error(ctx, TL_ERR_INVALID_ARG, "%s: %lld tokens for %d sequences need token_seq", who, (long long)tokens, c->n_seqs);
-  // positions are int32, and an offset inside a page too
-  if (int64_t(c->max_pages) * c->page_size > INT32_MAX || int64_t(c->n_kv_heads) * c->page_size * c->head_dim > INT32_MAX || tokens > INT32_MAX)
-    return tl_set_error(ctx, TL_ERR_UNSUPPORTED, "%s: positions, a page's elements and tokens are limited to 2^31 - 1", who);
+  // positions are int32 (a tile behind the last one too), and an offset inside a page
+  if (int64_t(c->max_pages) * c->page_size > INT32_MAX - 64 || int64_t(c->n_kv_heads) * c->page_size * c->head_dim > INT32_MAX || tokens > INT32_MAX)
+    return tl_set_error(ctx, TL_ERR_UNSUPPORTED, "%s: positions (2^31 - 64), a page's elements and tokens are limited to 2^31", who);
   return TL_OK;
 }
 

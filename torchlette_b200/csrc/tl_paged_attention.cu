@@ -32,7 +32,7 @@
 
 namespace {
 
-constexpr int kWarps = 4, kConsumers = 32 * kWarps, kThreads = kConsumers + 32, kGroup = 16, kMaxStages = 24;
+constexpr int kGroup = 16, kMaxStages = 24;
 
 struct PagedArgs {
   const void *q, *k_pages, *v_pages;
@@ -42,7 +42,7 @@ struct PagedArgs {
   int64_t qt, qh, n_pages;
   int32_t tokens, n_heads, n_kv_heads, rep, head_dim, page_size, n_seqs, max_pages, window, row_tiles, least_units, stages;
   TlDivide page_div;
-  float scale, softcap;
+  float scale, softcap, cap_exp;
   int *status, *wait_status;
   float* slots;        // [2 * CTAs] parts of tokens
   unsigned* arrivals;  // [3 * CTAs], zero between launches: CTAs of a group that have left their part, groups of a token
@@ -55,7 +55,8 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
 __device__ __forceinline__ void copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
+template <class Tile> constexpr int kConsumers = 32 * Tile::WARPS;
+template <class Tile> __device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers<Tile>) : "memory"); }
 __device__ __forceinline__ void ldmatrix4(uint32_t at, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
@@ -95,7 +96,7 @@ struct Cursor {
   Token k;
   template <int KEYS> __device__ __forceinline__ void open(const PagedArgs& p) {
     k = token_of(p, t, false);
-    n = tl_units(k.lo / KEYS * KEYS, k.hi, KEYS);
+    n = tl_tiles(k.lo, k.hi, KEYS);
   }
   __device__ __forceinline__ void head(const PagedArgs& p) {
     if (p.row_tiles == 1) { kvh = seg; tile = 0; }
@@ -150,6 +151,14 @@ __device__ __noinline__ void row_again(const PagedArgs& p, const Token& k, int p
   if (d0 + lane < p.head_dim) reinterpret_cast<AT*>(p.out)[(int64_t(t) * p.n_heads + h) * p.head_dim + d0 + lane] = DT<AT>::from_f32(o / sum);
 }
 
+// c tanh(x / c) = c - 2 c / (1 + exp(2 x / c)), scale = 2 log2(e) / c.  Off by a few 2^-23 c: a score's absolute error is its probability's relative one,
+// far below the output's own rounding in 16 bits.  (tanhf's two branches were a third of the kernel's instructions.)
+__device__ __forceinline__ float cap(float x, float c, float scale) {
+  float t;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(x * scale));
+  return fmaf(-2.f * c, __fdividef(1.f, 1.f + t), c);
+}
+
 // Probabilities are held times 2^10 in f16: the low term of their split stays clear of f16's subnormals.
 template <typename AT> constexpr float kProbBias = 0.f;
 template <> constexpr float kProbBias<__half> = 10.f;
@@ -159,7 +168,7 @@ template <> constexpr float kProbBias<__half> = 10.f;
 template <typename AT_, int DPAD_, int NT>
 struct MmaTile {
   using AT = AT_;
-  static constexpr int DPAD = DPAD_, ROWS = 8 * NT, KEYS = 16, TERMS = ProbSplit<AT>::kTerms, CTAS = DPAD * NT > 128 ? 1 : 2;
+  static constexpr int DPAD = DPAD_, ROWS = 8 * NT, KEYS = 16, TERMS = ProbSplit<AT>::kTerms, CTAS = DPAD * NT > 128 ? 1 : 2, WARPS = 8 / CTAS;
   static constexpr bool kRedo = true;  // infinite values need it
   uint32_t q[NT][DPAD / 16][2];
   float o[NT][DPAD / 16][4], m[NT][2], l[NT][2], slope[NT][2];
@@ -222,7 +231,7 @@ struct MmaTile {
         float x;
         if (OPTIONS) {
           x = s[nt][e] * p.scale;
-          if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
+          if (p.softcap > 0.f) x = cap(x, p.softcap, p.cap_exp);
           x = fmaf(slope[nt][e & 1], float(behind + key), x * kLog2e);
         } else {
           x = s[nt][e] * (p.scale * kLog2e);
@@ -323,12 +332,12 @@ template <int N, int BIT = 16> __device__ __forceinline__ float sum_exchange(con
 template <int DPAD_, int ROWS_>
 struct F32Tile {
   using AT = float;
-  static constexpr int DPAD = DPAD_, ROWS = ROWS_, KEYS = 8, E = DPAD / 32, CTAS = DPAD * ROWS > 512 ? 1 : 2;
+  static constexpr int DPAD = DPAD_, ROWS = ROWS_, KEYS = 8, E = DPAD / 32, CTAS = DPAD * ROWS > 512 ? 1 : 2, WARPS = 8 / CTAS;
   static constexpr bool kRedo = false;
   static constexpr int kSets = ROWS * KEYS > 32 ? ROWS * KEYS / 32 : 1, kN = ROWS * KEYS / kSets;  // kN values are summed at once
   static constexpr int kRowsOfSet = ROWS / kSets, kLog = kN == 32 ? 5 : kN == 16 ? 4 : 3;
-  float q[ROWS][E], o[ROWS][E], m[ROWS], l[ROWS];  // m: the same in all lanes; l: a lane's own
-  float slope[kSets];
+  float q[ROWS][E], o[ROWS][E];
+  float m[kSets], l[kSets], slope[kSets];  // of the row whose score this lane ends up with: its maximum, and the sum over this lane's keys
 
   __device__ __forceinline__ void begin(const PagedArgs& p, int t, int kvh, int tile) {
     const int lane = threadIdx.x & 31;
@@ -341,11 +350,11 @@ struct F32Tile {
         q[r][e] = row < p.rep && lane * E + e < p.head_dim ? __ldg(qp + e) : 0.f;
         o[r][e] = 0.f;
       }
-      m[r] = -INFINITY;
-      l[r] = 0.f;
     }
 #pragma unroll
     for (int s = 0; s < kSets; ++s) {
+      m[s] = -INFINITY;
+      l[s] = 0.f;
       const int row = tile * ROWS + s * kRowsOfSet + (lane >> (5 - kLog)) / KEYS;
       slope[s] = p.slopes && row < p.rep ? p.slopes[kvh * p.rep + row] * kLog2e : 0.f;
     }
@@ -397,22 +406,20 @@ struct F32Tile {
       float top = x;  // over the keys of a row: lanes that differ in the key's bits
 #pragma unroll
       for (int b = 1 << (5 - kLog); b < KEYS << (5 - kLog); b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+      const float nm = fmaxf(m[s], top);
+      if (__any_sync(0xffffffffu, nm != m[s])) {
+        const float f = nm == m[s] ? 1.f : exp2f(m[s] - nm);
+        m[s] = nm;
+        l[s] *= f;
 #pragma unroll
-      for (int i = 0; i < kRowsOfSet; ++i) {
-        const int r = s * kRowsOfSet + i;
-        const float nm = fmaxf(m[r], __shfl_sync(0xffffffffu, top, (i * KEYS) << (5 - kLog)));
-        if (nm != m[r]) {  // the same in all lanes
-          const float f = exp2f(m[r] - nm);
-          m[r] = nm;
-          l[r] *= f;
+        for (int i = 0; i < kRowsOfSet; ++i) {
+          const float g = __shfl_sync(0xffffffffu, f, (i * KEYS) << (5 - kLog));
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[r][e] *= f;
+          for (int e = 0; e < E; ++e) o[s * kRowsOfSet + i][e] *= g;
         }
       }
-      float mm = m[s * kRowsOfSet];
-#pragma unroll
-      for (int i = 1; i < kRowsOfSet; ++i) mm = (lane >> (5 - kLog)) / KEYS == i ? m[s * kRowsOfSet + i] : mm;
-      pr[s] = mm == -INFINITY ? 0.f : exp2f(x - mm);
+      pr[s] = nm == -INFINITY ? 0.f : exp2f(x - nm);
+      l[s] += pr[s];
     }
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
@@ -421,7 +428,6 @@ struct F32Tile {
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         const float w = __shfl_sync(0xffffffffu, pr[r / kRowsOfSet], ((r % kRowsOfSet) * KEYS + j) << (5 - kLog));
-        l[r] += w;  // all lanes hold the whole sum
 #pragma unroll
         for (int e = 0; e < E; ++e) o[r][e] = fmaf(w, v[e], o[r][e]);
       }
@@ -430,12 +436,18 @@ struct F32Tile {
   __device__ __forceinline__ void end(float* wm, float* wl, float* wo, int pitch, int rows) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
+    for (int s = 0; s < kSets; ++s) {
+      float v = l[s];
+#pragma unroll
+      for (int b = 1 << (5 - kLog); b < KEYS << (5 - kLog); b <<= 1) v += __shfl_xor_sync(0xffffffffu, v, b);
+      const int r = s * kRowsOfSet + (lane >> (5 - kLog)) / KEYS;
+      if ((lane & ((KEYS << (5 - kLog)) - 1)) == 0 && r < rows) { wm[r] = m[s]; wl[r] = v; }
+    }
+#pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (r < rows) {
-        if (lane == 0) { wm[r] = m[r]; wl[r] = l[r]; }
+      if (r < rows)
 #pragma unroll
         for (int e = 0; e < E; ++e) wo[r * pitch + lane * E + e] = o[r][e];
-      }
   }
 };
 
@@ -443,10 +455,10 @@ struct F32Tile {
 template <class Tile> constexpr int kBoxBytes = Tile::KEYS * 128;
 template <class Tile> constexpr int kBoxes = Tile::DPAD * int(sizeof(typename Tile::AT)) / 128;
 template <class Tile> constexpr int kStageBytes = 2 * kBoxes<Tile> * kBoxBytes<Tile>;
-// Behind the ring: [4][rows] maxima, [4][rows] sums and [4][rows][DPAD + 4] outputs of the consumer warps (the pitch keeps the lanes of a quad in
+// Behind the ring: [warps][rows][DPAD + 4] outputs, [warps][rows] maxima and [warps][rows] sums of the consumer warps (the pitch keeps the lanes of a quad in
 // banks of their own), which join() uses too.
 template <class Tile> constexpr int kPitch = Tile::DPAD + 4;
-template <class Tile> constexpr int area_bytes(int rows) { return kWarps * rows * (2 + kPitch<Tile>) * int(sizeof(float)); }
+template <class Tile> constexpr int area_bytes(int rows) { return Tile::WARPS * rows * (2 + kPitch<Tile>) * int(sizeof(float)); }
 // A part in scratch: [ROWS][DPAD] outputs, then [ROWS] maxima and [ROWS] sums; whole 16-byte vectors
 template <class Tile> __host__ __device__ constexpr int slot_floats() { return Tile::ROWS * Tile::DPAD + (2 * Tile::ROWS + 3) / 4 * 4; }
 template <class Tile> constexpr int kSlotMax = Tile::ROWS * Tile::DPAD;
@@ -459,7 +471,7 @@ __device__ __forceinline__ int slot_of(int first, int i) { return 2 * (first + i
 template <class Tile> __device__ void join(const float* slots, int first, int from, int step, int count, int rows, float* area) {
   float *maxima = area + rows * Tile::DPAD, *sums = maxima + rows, *factor = sums + rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < rows; r += kWarps) {
+  for (int r = warp; r < rows; r += Tile::WARPS) {
     float mx = -INFINITY, sum = 0.f;
     const float* at = slots + int64_t(slot_of(first, from + min(lane, count - 1) * step)) * slot_floats<Tile>() + r;
     if (lane < count) { mx = __ldcg(at + kSlotMax<Tile>); sum = __ldcg(at + kSlotSum<Tile>); }
@@ -473,27 +485,34 @@ template <class Tile> __device__ void join(const float* slots, int first, int fr
     if (lane < count) factor[r * count + lane] = f;
     if (lane == 0) { maxima[r] = top; sums[r] = sum; }
   }
-  consumers_meet();
-  for (int e = threadIdx.x * 4; e < rows * Tile::DPAD; e += kConsumers * 4) {
+  consumers_meet<Tile>();
+  for (int e = threadIdx.x * 4; e < rows * Tile::DPAD; e += kConsumers<Tile> * 4) {
     const int r = e / Tile::DPAD;
-    const float* at = slots + e;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = 0; i < count; ++i) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(at + int64_t(slot_of(first, from + i * step)) * slot_floats<Tile>()));
-      const float f = factor[r * count + i];
-      a.x = fmaf(f, v.x, a.x); a.y = fmaf(f, v.y, a.y); a.z = fmaf(f, v.z, a.z); a.w = fmaf(f, v.w, a.w);
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += 8) {  // eight loads together
+      float4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = __ldcg(reinterpret_cast<const float4*>(slots + int64_t(slot_of(first, from + min(i0 + i, count - 1) * step)) * slot_floats<Tile>() + e));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= count) break;
+        const float f = factor[r * count + i0 + i];
+        a.x = fmaf(f, v[i].x, a.x); a.y = fmaf(f, v[i].y, a.y); a.z = fmaf(f, v[i].z, a.z); a.w = fmaf(f, v[i].w, a.w);
+      }
     }
     *reinterpret_cast<float4*>(area + e) = a;
   }
-  consumers_meet();
+  consumers_meet<Tile>();
 }
 
 template <class Tile, bool OPTIONS, bool TMA>
-__global__ void __launch_bounds__(kThreads, Tile::CTAS)
+__global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     paged_attention_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using AT = typename Tile::AT;
-  constexpr int DPAD = Tile::DPAD, KEYS = Tile::KEYS, kHalf = kStageBytes<Tile> / 2, kPerChunk = 16 / int(sizeof(AT));
+  constexpr int DPAD = Tile::DPAD, KEYS = Tile::KEYS, WARPS = Tile::WARPS, kThreads = 32 + kConsumers<Tile>;
+  constexpr int kHalf = kStageBytes<Tile> / 2, kPerChunk = 16 / int(sizeof(AT));
   constexpr uint32_t kAll = (1u << KEYS) - 1;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
@@ -514,76 +533,108 @@ __global__ void __launch_bounds__(kThreads, Tile::CTAS)
     for (int i = threadIdx.x; i < p.stages * (kStageBytes<Tile> / 16); i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  __syncthreads();
   tl_pdl_wait();
 
-  // Tokens that see nothing, and how many tiles the others have
-  const int segs = p.n_kv_heads * p.row_tiles, chunk = (p.tokens + kThreads - 1) / kThreads;
-  const int t_first = min(p.tokens, int(threadIdx.x) * chunk), t_end = min(p.tokens, t_first + chunk);
-  auto tiles_of = [&](const Token& k) { return tl_units(k.lo / KEYS * KEYS, k.hi, KEYS); };
+  // What all tokens cost, and where this CTA's share begins: by every warp for itself where tokens are few, else by the threads together
+  const int segs = p.n_kv_heads * p.row_tiles;
+  const bool wide = p.tokens > 256;
+  const int id = wide ? int(threadIdx.x) : lane, chunk = (p.tokens + (wide ? kThreads : 32) - 1) / (wide ? kThreads : 32);
+  const int t_first = min(p.tokens, id * chunk), t_end = min(p.tokens, t_first + chunk);
+  auto cost_of = [&](int t) {
+    const Token k = token_of(p, t, false);
+    const int n = tl_tiles(k.lo, k.hi, KEYS);
+    return n ? n + kLead : 0;
+  };
   long long mine = 0;
-  for (int t = t_first; t < t_end; ++t) mine += tiles_of(token_of(p, t, t % int(gridDim.x) == cta));
-  for (int t = cta; t < p.tokens; t += int(gridDim.x))
-    if (token_of(p, t, false).hi == 0)
-      for (int e = threadIdx.x; e < p.n_heads * p.head_dim; e += kThreads)
-        reinterpret_cast<AT*>(p.out)[int64_t(t) * p.n_heads * p.head_dim + e] = DT<AT>::from_f32(0.f);
-  long long to = mine;
+  for (int t = t_first; t < t_end; ++t) mine += cost_of(t);
+  long long to = mine, whole;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long v = __shfl_up_sync(0xffffffffu, to, o);
     if (lane >= o) to += v;
   }
-  if (lane == 31) scan[warp] = to;
-  __syncthreads();
-  long long whole = 0;
+  whole = __shfl_sync(0xffffffffu, to, 31);
+  if (wide) {
+    if (lane == 31) scan[warp] = to;
+    __syncthreads();
+    whole = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) to += scan[w];
-    whole += scan[w];
-  }
-  const long long units = whole * segs;
-  const int ctas = tl_share_ctas(units, int(gridDim.x), p.least_units);
-  if (units == 0 || cta >= ctas) return;
-  const long long begin = tl_share_begin(units, ctas, cta), end = tl_share_begin(units, ctas, cta + 1);
-  if ((to - mine) * segs <= begin && begin < to * segs) {  // one thread's
-    long long at = (to - mine) * segs;
-    for (int t = t_first; t < t_end; ++t) {
-      const long long n = (long long)(tiles_of(token_of(p, t, false))) * segs;
-      if (begin < at + n) {
-        found_token = t;
-        found_begin = begin - at;
-        break;
-      }
-      at += n;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) to += scan[w];
+      whole += scan[w];
     }
   }
-  __syncthreads();
+  for (int t = cta; t < p.tokens; t += int(gridDim.x))  // tokens that see nothing
+    if (token_of(p, t, threadIdx.x == 0).hi == 0)
+      for (int e = threadIdx.x; e < p.n_heads * p.head_dim; e += kThreads)
+        reinterpret_cast<AT*>(p.out)[int64_t(t) * p.n_heads * p.head_dim + e] = DT<AT>::from_f32(0.f);
+  if (whole == 0) return;
+  const TlShares shares = tl_shares(whole * segs, int(gridDim.x), p.least_units, (long long)(p.tokens) * segs);
+  if (cta >= shares.ctas) return;
+  const long long begin = tl_share_begin(shares, cta), end = tl_share_begin(shares, cta + 1);
   Cursor c;
-  c.t = found_token;
+  long long into = 0;  // how far the share's begin lies in the units of its token
+  const bool found = (to - mine) * segs <= begin && begin < to * segs;  // one thread's
+  c.t = 0;
+  if (found) {
+    into = begin - (to - mine) * segs;
+    for (c.t = t_first; c.t < t_end; ++c.t) {
+      const long long n = (long long)(cost_of(c.t)) * segs;
+      if (into < n) break;
+      into -= n;
+    }
+  }
+  if (wide) {
+    if (found) { found_token = c.t; found_begin = into; }
+    __syncthreads();
+    c.t = found_token;
+    into = found_begin;
+  } else {
+    const int from = __ffs(__ballot_sync(0xffffffffu, found)) - 1;
+    c.t = __shfl_sync(0xffffffffu, c.t, from);
+    into = __shfl_sync(0xffffffffu, into, from);
+  }
   c.template open<KEYS>(p);
-  c.seg = int(found_begin / c.n);
-  c.u = int(found_begin - (long long)(c.seg) * c.n);
+  c.seg = int(tl_quotient(into, c.n + kLead));
   c.head(p);
+  long long tile0 = begin - (into - (long long)(c.seg) * (c.n + kLead)) + kLead;  // the unit of the part's first tile
+  // The part's tiles in the share are [c.u, stop)
+  int stop;
+  auto clip = [&]() {
+    c.u = int(max(0ll, begin - tile0));
+    stop = int(min((long long)(c.n), end - tile0));
+  };
+  auto advance = [&]() {  // to the next part; false: the share ends here
+    tile0 += c.n + kLead;
+    if (tile0 >= end) return false;
+    c.template next<KEYS>(p);
+    clip();
+    return true;
+  };
+  clip();
 
-  if (warp == kWarps) {
+  if (warp == WARPS) {
     // ---- the producer.  A lane looks up a tile's page (cp.async: a row's) a batch before it is copied, so that the table is read on the way.
     constexpr int kBatch = TMA ? 32 : 1;
     struct Batch {
       int n, key0, kvh, key, page;  // n tiles from key0 on; this lane's key and its page
       Token k;
     };
-    long long left = end - begin;
+    bool more = true;
     auto look_up = [&]() {
       Batch b;
-      b.n = int(min((long long)(min(kBatch, c.n - c.u)), left));
+      b.n = 0;
+      while (more && c.u >= stop) more = advance();
+      if (!more) return b;
+      b.n = min(kBatch, stop - c.u);
       b.k = c.k;
       b.kvh = c.kvh;
       b.key0 = c.template first_key<KEYS>(c.u);
       b.key = b.key0 + (TMA ? lane * KEYS : lane);
       b.page = -1;
       if (TMA ? lane < b.n : lane < KEYS && b.key >= b.k.lo && b.key < b.k.hi) b.page = __ldg(p.page_table + b.k.seq * p.max_pages + tl_divide(b.key, p.page_div));
-      left -= b.n;
       c.u += b.n;
-      if (c.u == c.n && left > 0) c.template next<KEYS>(p);
       return b;
     };
     Batch now = look_up();
@@ -591,9 +642,7 @@ __global__ void __launch_bounds__(kThreads, Tile::CTAS)
     uint32_t parity = 1;  // of the phase before the first: the ring is empty
     bool ok = true;
     while (now.n > 0 && ok) {
-      Batch then;
-      then.n = 0;
-      if (left > 0) then = look_up();
+      const Batch then = look_up();
       const bool wanted = TMA ? lane < now.n : lane < KEYS && now.key >= now.k.lo && now.key < now.k.hi, there = wanted && !tl_bad_page(now.page, p.n_pages);
       if (wanted && !there) atomicOr(p.status, kBadPage);
       const int in_page = now.key - tl_divide(now.key, p.page_div) * p.page_size;
@@ -653,116 +702,145 @@ __global__ void __launch_bounds__(kThreads, Tile::CTAS)
     return;
   }
 
-  // ---- the consumers: warp w takes the share's tiles w, w + 4, ...
+  // ---- the consumers: warp w takes the share's tiles w, w + WARPS, ...
   float* area = reinterpret_cast<float*>(sm + p.stages * kStageBytes<Tile>);
-  int stage = warp, parity = 0;
+  int stage = warp, parity = 0, turn = warp;  // turn: how many of the share's tiles lie before this warp's next, from the part's first in the share
   while (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
-  bool ok = true;
-  long long next = begin + warp, at = begin;  // this warp's next tile; the first of the current token's and group's in the share
+  bool ok = true, more = true, met = true;
   Tile tile;
-  while (at < end) {
-    tile.begin(p, c.t, c.kvh, c.tile);
-    const long long seg_begin = at - c.u, seg_end = seg_begin + c.n, stop = min(seg_end, end);
-    for (; next < stop; next += kWarps) {
-      if (ok && !mbar_wait_all(&full[stage], parity, &abort_flag)) {
-        ok = false;
-        if (lane == 0) { atomicExch(&abort_flag, 1); atomicExch(p.wait_status, TL_DEV_TIMEOUT_FULL); }
-      }
-      if (ok) {
-        const uint32_t seen = seen_of[stage], ks = smem_u32(sm + stage * kStageBytes<Tile>);
-        if (seen) {
-          if (TMA && seen != kAll) {  // values that do not count, whatever they are
-            for (int i = lane; i < KEYS * kBoxes<Tile> * 8; i += 32) {
-              const int r = (i >> 3) % KEYS;
-              if (!((seen >> r) & 1)) reinterpret_cast<uint4*>(sm + stage * kStageBytes<Tile> + kHalf)[i] = make_uint4(0, 0, 0, 0);
+  while (more) {
+    if (c.u < stop) {
+      tile.begin(p, c.t, c.kvh, c.tile);
+      const bool starts = c.u == 0, ends = stop == c.n;
+      int i = c.u + turn;
+      for (; i < stop; i += WARPS) {
+        if (ok && !mbar_wait_all(&full[stage], parity, &abort_flag)) {
+          ok = false;
+          if (lane == 0) { atomicExch(&abort_flag, 1); atomicExch(p.wait_status, TL_DEV_TIMEOUT_FULL); }
+        }
+        if (ok) {
+          const uint32_t seen = seen_of[stage], ks = smem_u32(sm + stage * kStageBytes<Tile>);
+          if (seen) {
+            if (TMA && seen != kAll) {  // values that do not count, whatever they are
+              for (int j = lane; j < KEYS * kBoxes<Tile> * 8; j += 32) {
+                const int r = (j >> 3) % KEYS;
+                if (!((seen >> r) & 1)) reinterpret_cast<uint4*>(sm + stage * kStageBytes<Tile> + kHalf)[j] = make_uint4(0, 0, 0, 0);
+              }
+              __syncwarp();
             }
-            __syncwarp();
+            tile.template take<OPTIONS>(p, ks, ks + kHalf, seen, c.template first_key<KEYS>(i) + 1 - c.k.hi);
+            if (TMA && seen != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
-          tile.template take<OPTIONS>(p, ks, ks + kHalf, seen, c.template first_key<KEYS>(int(next - seg_begin)) + 1 - c.k.hi);
-          if (TMA && seen != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[stage]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[stage]);
+        stage += WARPS;
+        while (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
       }
-      stage += kWarps;
-      while (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
-    }
+      turn = i - stop;
 
-    // The last tile of this token and group, or of this CTA's share
-    const int rows = min(Tile::ROWS, p.rep - c.tile * Tile::ROWS), h0 = c.kvh * p.rep + c.tile * Tile::ROWS;
-    float *wm = area, *wl = wm + kWarps * rows, *wo = wl + kWarps * rows;
-    const bool starts = seg_begin >= begin, ends = seg_end <= end;
-    tile.end(wm + warp * rows, wl + warp * rows, wo + warp * rows * kPitch<Tile>, kPitch<Tile>, rows);
-    consumers_meet();
-    auto store = [&](int r, int d, float v) {  // a warp's 32 values are one row's
-      if (Tile::kRedo && __any_sync(0xffffffffu, d < p.head_dim && !isfinite(v))) {
-        row_again<AT>(p, c.k, c.k.hi - 1, c.t, h0 + r, c.kvh, d & ~31);
-      } else if (d < p.head_dim) {
-        reinterpret_cast<AT*>(p.out)[(int64_t(c.t) * p.n_heads + h0 + r) * p.head_dim + d] = DT<AT>::from_f32(v);
-      }
-    };
-    float* slot = p.slots + int64_t(2 * cta + (starts ? 1 : 0)) * slot_floats<Tile>();
-    for (int e = threadIdx.x; e < rows * DPAD; e += kConsumers) {
-      const int r = e / DPAD, d = e - r * DPAD;
-      float top = -INFINITY;
+      // The end of this part, or of this CTA's share of it
+      const int rows = min(Tile::ROWS, p.rep - c.tile * Tile::ROWS), h0 = c.kvh * p.rep + c.tile * Tile::ROWS;
+      float *wo = area, *wm = wo + WARPS * rows * kPitch<Tile>, *wl = wm + WARPS * rows;
+      if (!met) consumers_meet<Tile>();  // the area is free again
+      met = false;
+      tile.end(wm + warp * rows, wl + warp * rows, wo + warp * rows * kPitch<Tile>, kPitch<Tile>, rows);
+      consumers_meet<Tile>();
+      // Four neighbouring values of a row by each thread
+      auto store = [&](int e, float4 o, float sum) {
+        const int r = e / DPAD, d = e - r * DPAD;
+        float v[4] = {o.x, o.y, o.z, o.w};
+        bool odd = false;
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) top = fmaxf(top, wm[i * rows + r]);
-      float sum = 0.f, o = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        const float mx = wm[i * rows + r], g = mx == -INFINITY ? 0.f : exp2f(mx - top);
-        sum = fmaf(wl[i * rows + r], g, sum);
-        o = fmaf(wo[(i * rows + r) * kPitch<Tile> + d], g, o);
-      }
-      if (starts && ends) {
-        store(r, d, sum == 0.f ? 0.f : o / sum);  // no key's page is there: nothing is seen
-      } else {
-        if (d == 0) { __stcg(slot + kSlotMax<Tile> + r, top); __stcg(slot + kSlotSum<Tile> + r, sum); }
-        __stcg(slot + e, o);
-      }
-    }
-    if (!(starts && ends)) {
-      // The token's CTAs are first .. first + count - 1.  Whoever comes last of a group of kGroup joins the group's parts, in the place of the first of
-      // them, and whoever ends the last group joins the groups'.
-      const int first = tl_share_owner(units, ctas, seg_begin), count = tl_share_owner(units, ctas, seg_end - 1) - first + 1;
-      const int group = (cta - first) / kGroup, groups = (count + kGroup - 1) / kGroup, members = min(kGroup, count - group * kGroup);
-      auto last_of = [&](unsigned* arrived, int of) {
-        __threadfence();
-        consumers_meet();
-        if (threadIdx.x == 0) {
-          is_last = atomicAdd(arrived, 1u) == unsigned(of) - 1;
-          if (is_last) *arrived = 0;  // for the next launch
+        for (int j = 0; j < 4; ++j) {
+          v[j] = sum == 0.f ? 0.f : v[j] / sum;  // no key's page is there: nothing is seen
+          odd |= !isfinite(v[j]);
         }
-        consumers_meet();
-        __threadfence();
-        return is_last != 0;
-      };
-      bool done = last_of(p.arrivals + slot_of(first, group * kGroup), members);
-      if (done) {
-        join<Tile>(p.slots, first, group * kGroup, 1, members, rows, area);
-        if (groups > 1) {
-          float* to_slot = p.slots + int64_t(slot_of(first, group * kGroup)) * slot_floats<Tile>();
-          for (int e = threadIdx.x; e < rows * DPAD; e += kConsumers) __stcg(to_slot + e, area[e]);
-          if (int(threadIdx.x) < rows) {
-            __stcg(to_slot + kSlotMax<Tile> + threadIdx.x, area[rows * DPAD + threadIdx.x]);
-            __stcg(to_slot + kSlotSum<Tile> + threadIdx.x, area[rows * DPAD + rows + threadIdx.x]);
+        if (d < p.head_dim) {
+          AT* to_at = reinterpret_cast<AT*>(p.out) + (int64_t(c.t) * p.n_heads + h0 + r) * p.head_dim + d;
+          if (sizeof(AT) == 4) {
+            *reinterpret_cast<float4*>(to_at) = make_float4(v[0], v[1], v[2], v[3]);
+          } else {
+            AT h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[j] = DT<AT>::from_f32(v[j]);
+            *reinterpret_cast<uint2*>(to_at) = *reinterpret_cast<const uint2*>(h);
           }
-          done = last_of(p.arrivals + 2 * gridDim.x + first, groups);
-          if (done) join<Tile>(p.slots, first, 0, kGroup, groups, rows, area);
+        }
+        return Tile::kRedo && odd && d < p.head_dim;
+      };
+      // After the stores of a warp's 128 values from e0 on: the rows' blocks of 32 that have one that is not finite, again
+      auto store_again = [&](uint32_t odd, int e0) {
+        if (!odd) return;
+        __syncwarp();
+        for (int b = 0; b < 4; ++b)
+          if ((odd >> (8 * b)) & 0xff) row_again<AT>(p, c.k, c.k.hi - 1, c.t, h0 + (e0 + 32 * b) / DPAD, c.kvh, (e0 + 32 * b) % DPAD);
+      };
+      float* slot = p.slots + int64_t(2 * cta + (starts ? 1 : 0)) * slot_floats<Tile>();
+      for (int e0 = warp * 128; e0 < rows * DPAD; e0 += WARPS * 128) {
+        const int e = e0 + 4 * lane, r = min(e, rows * DPAD - 1) / DPAD, d = e - r * DPAD;
+        const bool here = e < rows * DPAD;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = -INFINITY, sum = 0.f;
+        if (here) {
+#pragma unroll
+          for (int i = 0; i < WARPS; ++i) top = fmaxf(top, wm[i * rows + r]);
+#pragma unroll
+          for (int i = 0; i < WARPS; ++i) {
+            const float mx = wm[i * rows + r], g = mx == -INFINITY ? 0.f : exp2f(mx - top);
+            const float4 w = *reinterpret_cast<const float4*>(wo + (i * rows + r) * kPitch<Tile> + d);
+            sum = fmaf(wl[i * rows + r], g, sum);
+            o.x = fmaf(w.x, g, o.x); o.y = fmaf(w.y, g, o.y); o.z = fmaf(w.z, g, o.z); o.w = fmaf(w.w, g, o.w);
+          }
+        }
+        if (starts && ends) {
+          const bool odd = here && store(e, o, sum);
+          store_again(__ballot_sync(0xffffffffu, odd), e0);
+        } else if (here) {
+          if (d == 0) { __stcg(slot + kSlotMax<Tile> + r, top); __stcg(slot + kSlotSum<Tile> + r, sum); }
+          __stcg(reinterpret_cast<float4*>(slot + e), o);
         }
       }
-      if (done)
-        for (int e = threadIdx.x; e < rows * DPAD; e += kConsumers) {
-          const int r = e / DPAD;
-          const float sum = area[rows * DPAD + rows + r];
-          store(r, e - r * DPAD, sum == 0.f ? 0.f : area[e] / sum);
+      if (!(starts && ends)) {
+        // The part's CTAs are first .. first + count - 1.  Whoever comes last of a group of kGroup joins what the group has left, in the place of the
+        // first of them, and whoever ends the last group joins the groups'.
+        const int first = tl_share_owner(shares, tile0), count = tl_share_owner(shares, tile0 + c.n - 1) - first + 1;
+        const int group = (cta - first) / kGroup, groups = (count + kGroup - 1) / kGroup, members = min(kGroup, count - group * kGroup);
+        auto last_of = [&](unsigned* arrived, int of) {
+          consumers_meet<Tile>();
+          if (threadIdx.x == 0) {
+            __threadfence();
+            is_last = atomicAdd(arrived, 1u) == unsigned(of) - 1;
+            if (is_last) *arrived = 0;  // for the next launch
+            __threadfence();
+          }
+          consumers_meet<Tile>();
+          return is_last != 0;
+        };
+        bool done = last_of(p.arrivals + slot_of(first, group * kGroup), members);
+        if (done) {
+          join<Tile>(p.slots, first, group * kGroup, 1, members, rows, area);
+          if (groups > 1) {
+            float* to_slot = p.slots + int64_t(slot_of(first, group * kGroup)) * slot_floats<Tile>();
+            for (int e = threadIdx.x * 4; e < rows * DPAD; e += kConsumers<Tile> * 4)
+              __stcg(reinterpret_cast<float4*>(to_slot + e), *reinterpret_cast<const float4*>(area + e));
+            if (int(threadIdx.x) < rows) {
+              __stcg(to_slot + kSlotMax<Tile> + threadIdx.x, area[rows * DPAD + threadIdx.x]);
+              __stcg(to_slot + kSlotSum<Tile> + threadIdx.x, area[rows * DPAD + rows + threadIdx.x]);
+            }
+            done = last_of(p.arrivals + 2 * gridDim.x + first, groups);
+            if (done) join<Tile>(p.slots, first, 0, kGroup, groups, rows, area);
+          }
         }
+        if (done)
+          for (int e0 = warp * 128; e0 < rows * DPAD; e0 += WARPS * 128) {
+            const int e = e0 + 4 * lane;
+            const bool odd = e < rows * DPAD && store(e, *reinterpret_cast<const float4*>(area + e), area[rows * DPAD + rows + e / DPAD]);
+            store_again(__ballot_sync(0xffffffffu, odd), e0);
+          }
+      }
     }
-    at = stop;
-    if (at < end) {
-      c.template next<KEYS>(p);
-      consumers_meet();  // the area is free again
-    }
+    more = advance();
   }
 }
 
@@ -777,7 +855,7 @@ cudaError_t launch(tl_ctx* ctx, PagedArgs& p, const CUtensorMap& k_map, const CU
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(std::min<int64_t>(int64_t(ctx->sm_count) * Tile::CTAS, std::max<int64_t>(1, most_units))));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(32 + kConsumers<Tile>);
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[1] = {tl_pdl_attribute()};
@@ -817,7 +895,7 @@ cudaError_t launch_f32(tl_ctx* ctx, PagedArgs& p, int64_t longest) {
 }
 
 // Parts of tokens for two CTAs an SM of the largest slot, and the arrivals: one size for all calls, so that no captured call's scratch is replaced.
-constexpr int kSlotFloats = 16 * 130, kLeastUnits = 16;
+constexpr int kSlotFloats = 16 * 130, kLeastUnits = 24;
 static_assert(slot_floats<MmaTile<__half, 64, 2>>() <= kSlotFloats && slot_floats<F32Tile<256, 4>>() <= kSlotFloats && slot_floats<F32Tile<128, 8>>() <= kSlotFloats, "slots");
 static_assert(slot_floats<MmaTile<__half, 256, 1>>() <= kSlotFloats && slot_floats<MmaTile<__half, 128, 2>>() <= kSlotFloats, "slots");
 int32_t secure_scratch(tl_ctx* ctx) {
@@ -870,7 +948,7 @@ int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32
   p.qt = q_token_stride; p.qh = q_head_stride; p.n_pages = cache->n_pages;
   p.tokens = int32_t(tokens); p.n_heads = int32_t(n_heads); p.n_kv_heads = cache->n_kv_heads; p.rep = int32_t(n_heads / cache->n_kv_heads);
   p.head_dim = cache->head_dim; p.page_size = cache->page_size; p.n_seqs = cache->n_seqs; p.max_pages = cache->max_pages;
-  p.window = window; p.scale = scale; p.softcap = softcap; p.least_units = kLeastUnits;
+  p.window = window; p.scale = scale; p.softcap = softcap; p.cap_exp = softcap > 0.f ? 2.f * kLog2e / softcap : 0.f; p.least_units = kLeastUnits;
   p.page_div = tl_divide_by(cache->page_size);
   p.status = ctx->dev_status + 1;
   p.wait_status = ctx->dev_status;
