@@ -42,10 +42,10 @@ TL_HD int64_t tl_quotient(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? 
 // CTAs that a call uses: a share of fewer than least_units does not pay for a CTA's fixed costs, unless it is a part by itself
 // (short sequences side by side rather than one after another); every share has a tile
 TL_HD TlShares tl_shares(int64_t units, int32_t most, int32_t least_units, int64_t parts) {
-  int64_t c = tl_quotient(units, least_units);
+  int64_t c = units / least_units;  // a constant where it is called
   if (c < parts) c = parts;
   if (c > most) c = most;
-  if (c * (kLead + 1) > units) c = tl_quotient(units, kLead + 1);
+  if (c * (kLead + 1) > units) c = units / (kLead + 1);
   if (c < 1) c = 1;
   const int64_t each = tl_quotient(units, c);
   return {units, each, int32_t(c), int32_t(units - each * c)};

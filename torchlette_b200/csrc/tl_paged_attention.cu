@@ -9,7 +9,7 @@
 // depends on a length, so that a captured call serves sequences that grow.  A producer warp looks up the pages, a batch of tiles ahead, and fills a ring of tiles
 // in shared memory across the borders of tokens and heads; four consumer warps take the tiles in turn, each with a softmax of its own, and
 // meet at the end of a token's keys.  Where a share ends inside a token's keys the CTA leaves maximum, sum and output in scratch, and whoever of that
-// token's CTAs comes last joins them in the order of the keys (in groups of 16 first, where they are many), so that no result depends on timing.
+// token's CTAs comes last joins them in the order of the keys (in groups of 12 first, where they are many), so that no result depends on timing.
 //
 // The ring.  Where a tile's rows are neighbours in a page (page_size a multiple of the tile), TMA boxes of 128-byte columns, 128-byte swizzle: an
 // instruction for each 2 KB.  Other page sizes: cp.async into the same layout, 16 bytes a lane.
@@ -32,7 +32,11 @@
 
 namespace {
 
-constexpr int kGroup = 16, kMaxStages = 24;
+#ifndef PA_CTAS
+#define PA_CTAS 2
+#define PA_WARPS 3
+#endif
+constexpr int kCtas = PA_CTAS, kConsumerWarps = PA_WARPS, kGroup = 12, kMaxStages = 48, kLeastUnits = 12;
 
 struct PagedArgs {
   const void *q, *k_pages, *v_pages;
@@ -40,8 +44,8 @@ struct PagedArgs {
   const int32_t *page_table, *positions, *token_seq;
   const float* slopes;
   int64_t qt, qh, n_pages;
-  int32_t tokens, n_heads, n_kv_heads, rep, head_dim, page_size, n_seqs, max_pages, window, row_tiles, least_units, stages;
-  TlDivide page_div;
+  int32_t tokens, n_heads, n_kv_heads, rep, head_dim, page_size, n_seqs, max_pages, window, row_tiles, stages;
+  TlDivide page_div, stage_div;
   float scale, softcap, cap_exp;
   int *status, *wait_status;
   float* slots;        // [2 * CTAs] parts of tokens
@@ -54,6 +58,25 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
 // Arrives once this thread's copies so far have landed
 __device__ __forceinline__ void copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// What is seen of a stage's tile (low half) and the lap of the ring that it belongs to (high half), written before the tile is asked for.  A parity wait passes
+// in the phase before the one that it means too, and a consumer may come to a stage before the lap in front of its own has landed there, since
+// the tiles in between are other warps'.  So it waits for its lap's word first: the producer writes it once the lap before has been consumed.
+__device__ __forceinline__ void publish(uint32_t* at, int lap, uint32_t seen) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(at)), "r"((uint32_t(lap) << 16) | seen) : "memory");
+}
+// By a whole warp; false: gave up
+__device__ __forceinline__ bool tile_ready(uint32_t* at, uint64_t* full, int lap, volatile int* abort_flag, uint32_t& seen) {
+  uint32_t word = 0;
+  bool here = false;
+  for (int it = 0; it < kWaitTimeoutIters && !here; ++it) {
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(word) : "r"(smem_u32(at)) : "memory");
+    here = word >> 16 == (uint32_t(lap) & 0xffffu);
+    if ((it & 63) == 63 && *abort_flag) break;
+  }
+  if (!__all_sync(0xffffffffu, here)) return false;
+  seen = word & 0xffffu;
+  return mbar_wait_all(full, lap & 1, abort_flag);
 }
 template <class Tile> constexpr int kConsumers = 32 * Tile::WARPS;
 template <class Tile> __device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers<Tile>) : "memory"); }
@@ -71,8 +94,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 
 // The keys that token t sees, [lo, hi) of sequence seq; none of them if it is not there.
 struct Token {
-  int32_t lo, hi;
-  int64_t seq;
+  int32_t lo, hi, seq;
 };
 __device__ __forceinline__ Token token_of(const PagedArgs& p, int t, bool report) {
   Token k{0, 0, 0};
@@ -128,7 +150,7 @@ __device__ __noinline__ void row_again(const PagedArgs& p, const Token& k, int p
   for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll 1
     for (int j = k.lo; j < k.hi; ++j) {
-      const int index = tl_divide(j, p.page_div), page = p.page_table[k.seq * p.max_pages + index];
+      const int index = tl_divide(j, p.page_div), page = p.page_table[int64_t(k.seq) * p.max_pages + index];
       if (tl_bad_page(page, p.n_pages)) continue;
       const int64_t at = tl_page_at(page, j - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim) + int64_t(kvh) * p.page_size * p.head_dim;
       const AT* kp = reinterpret_cast<const AT*>(p.k_pages) + at;
@@ -168,7 +190,7 @@ template <> constexpr float kProbBias<__half> = 10.f;
 template <typename AT_, int DPAD_, int NT>
 struct MmaTile {
   using AT = AT_;
-  static constexpr int DPAD = DPAD_, ROWS = 8 * NT, KEYS = 16, TERMS = ProbSplit<AT>::kTerms, CTAS = DPAD * NT > 128 ? 1 : 2, WARPS = 8 / CTAS;
+  static constexpr int DPAD = DPAD_, ROWS = 8 * NT, KEYS = 16, TERMS = ProbSplit<AT>::kTerms, CTAS = kCtas, WARPS = kConsumerWarps;
   static constexpr bool kRedo = true;  // infinite values need it
   uint32_t q[NT][DPAD / 16][2];
   float o[NT][DPAD / 16][4], m[NT][2], l[NT][2], slope[NT][2];
@@ -310,6 +332,33 @@ struct MmaTile {
         }
       }
   }
+  // The rows' outputs straight from the registers, where the warp's keys are all there are; true if one of this lane's is not finite
+  __device__ __forceinline__ bool finish(AT* out, int dim, int rows) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    bool odd = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = l[nt][e];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        const float inv = v == 0.f ? 0.f : 1.f / v;
+        const int r = nt * 8 + 2 * c + e;
+        if (r < rows) {
+#pragma unroll
+          for (int i = 0; i < DPAD / 8; ++i) {
+            const float x = o[nt][i >> 1][e + 2 * (i & 1)] * inv;
+            if (8 * i < dim) {
+              out[r * dim + 8 * i + g] = DT<AT>::from_f32(x);
+              odd |= !isfinite(x);
+            }
+          }
+        }
+      }
+    return odd;
+  }
 };
 
 // Sums N values over the warp, each lane ending with the one of number lane_value<N>(lane): at every step a lane keeps half of its values and hands
@@ -332,7 +381,7 @@ template <int N, int BIT = 16> __device__ __forceinline__ float sum_exchange(con
 template <int DPAD_, int ROWS_>
 struct F32Tile {
   using AT = float;
-  static constexpr int DPAD = DPAD_, ROWS = ROWS_, KEYS = 8, E = DPAD / 32, CTAS = DPAD * ROWS > 512 ? 1 : 2, WARPS = 8 / CTAS;
+  static constexpr int DPAD = DPAD_, ROWS = ROWS_, KEYS = 8, E = DPAD / 32, CTAS = kCtas, WARPS = kConsumerWarps;
   static constexpr bool kRedo = false;
   static constexpr int kSets = ROWS * KEYS > 32 ? ROWS * KEYS / 32 : 1, kN = ROWS * KEYS / kSets;  // kN values are summed at once
   static constexpr int kRowsOfSet = ROWS / kSets, kLog = kN == 32 ? 5 : kN == 16 ? 4 : 3;
@@ -449,6 +498,25 @@ struct F32Tile {
 #pragma unroll
         for (int e = 0; e < E; ++e) wo[r * pitch + lane * E + e] = o[r][e];
   }
+  __device__ __forceinline__ bool finish(float* out, int dim, int rows) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) {
+      float v = l[s];
+#pragma unroll
+      for (int b = 1 << (5 - kLog); b < KEYS << (5 - kLog); b <<= 1) v += __shfl_xor_sync(0xffffffffu, v, b);
+      const float inv = v == 0.f ? 0.f : 1.f / v;
+#pragma unroll
+      for (int i = 0; i < kRowsOfSet; ++i) {
+        const float f = __shfl_sync(0xffffffffu, inv, (i * KEYS) << (5 - kLog));
+        const int r = s * kRowsOfSet + i;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (r < rows && lane * E + e < dim) out[r * dim + lane * E + e] = o[r][e] * f;
+      }
+    }
+    return false;
+  }
 };
 
 // A stage of the ring: a tile's keys, then its values, each in boxes of KEYS rows of 128 bytes (16-byte chunk c of row r at c ^ (r & 7)).
@@ -471,10 +539,17 @@ __device__ __forceinline__ int slot_of(int first, int i) { return 2 * (first + i
 template <class Tile> __device__ void join(const float* slots, int first, int from, int step, int count, int rows, float* area) {
   float *maxima = area + rows * Tile::DPAD, *sums = maxima + rows, *factor = sums + rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto part = [&](int i) { return slots + int64_t(slot_of(first, from + min(i, count - 1) * step)) * slot_floats<Tile>(); };
+  // the first outputs are on their way while the factors are worked out
+  constexpr int kLoads = 12;
+  const int e_first = threadIdx.x * 4;
+  float4 v[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+    if (e_first < rows * Tile::DPAD) v[i] = __ldcg(reinterpret_cast<const float4*>(part(i) + e_first));
   for (int r = warp; r < rows; r += Tile::WARPS) {
     float mx = -INFINITY, sum = 0.f;
-    const float* at = slots + int64_t(slot_of(first, from + min(lane, count - 1) * step)) * slot_floats<Tile>() + r;
-    if (lane < count) { mx = __ldcg(at + kSlotMax<Tile>); sum = __ldcg(at + kSlotSum<Tile>); }
+    if (lane < count) { mx = __ldcg(part(lane) + kSlotMax<Tile> + r); sum = __ldcg(part(lane) + kSlotSum<Tile> + r); }
     float top = mx;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -486,21 +561,20 @@ template <class Tile> __device__ void join(const float* slots, int first, int fr
     if (lane == 0) { maxima[r] = top; sums[r] = sum; }
   }
   consumers_meet<Tile>();
-  for (int e = threadIdx.x * 4; e < rows * Tile::DPAD; e += kConsumers<Tile> * 4) {
+  for (int e = e_first; e < rows * Tile::DPAD; e += kConsumers<Tile> * 4) {
     const int r = e / Tile::DPAD;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int i0 = 0; i0 < count; i0 += 8) {  // eight loads together
-      float4 v[8];
+    for (int i0 = 0; i0 < count; i0 += kLoads) {
+      if (i0 > 0 || e != e_first)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = __ldcg(reinterpret_cast<const float4*>(slots + int64_t(slot_of(first, from + min(i0 + i, count - 1) * step)) * slot_floats<Tile>() + e));
+        for (int i = 0; i < kLoads; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(part(i0 + i) + e));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i0 + i >= count) break;
-        const float f = factor[r * count + i0 + i];
-        a.x = fmaf(f, v[i].x, a.x); a.y = fmaf(f, v[i].y, a.y); a.z = fmaf(f, v[i].z, a.z); a.w = fmaf(f, v[i].w, a.w);
-      }
+      for (int i = 0; i < kLoads; ++i)
+        if (i0 + i < count) {
+          const float f = factor[r * count + i0 + i];
+          a.x = fmaf(f, v[i].x, a.x); a.y = fmaf(f, v[i].y, a.y); a.z = fmaf(f, v[i].z, a.z); a.w = fmaf(f, v[i].w, a.w);
+        }
     }
     *reinterpret_cast<float4*>(area + e) = a;
   }
@@ -520,13 +594,14 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
   __shared__ long long found_begin, scan[kThreads / 32];
   __shared__ int found_token, is_last, abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = int(blockIdx.x);
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], TMA ? 1 : 33);  // cp.async: every lane's copies, and the word of what is seen
-      mbar_init(&empty[s], 1);
-    }
-    abort_flag = 0;
+  if (int(threadIdx.x) < p.stages) {
+    mbar_init(&full[threadIdx.x], TMA ? 1 : 33);  // cp.async: every lane's copies, and the word of what is seen
+    mbar_init(&empty[threadIdx.x], 1);
+    seen_of[threadIdx.x] = 0xffff0000u;  // no lap's
     mbar_fence_init();
+  }
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
     if (TMA) { tma_prefetch_desc(&k_map); tma_prefetch_desc(&v_map); }
   }
   if (p.head_dim < DPAD) {  // no copy writes the padding: it is zero from here on
@@ -541,13 +616,18 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
   const bool wide = p.tokens > 256;
   const int id = wide ? int(threadIdx.x) : lane, chunk = (p.tokens + (wide ? kThreads : 32) - 1) / (wide ? kThreads : 32);
   const int t_first = min(p.tokens, id * chunk), t_end = min(p.tokens, t_first + chunk);
-  auto cost_of = [&](int t) {
-    const Token k = token_of(p, t, false);
+  auto cost_of = [&](const Token& k) {
     const int n = tl_tiles(k.lo, k.hi, KEYS);
     return n ? n + kLead : 0;
   };
   long long mine = 0;
-  for (int t = t_first; t < t_end; ++t) mine += cost_of(t);
+  bool nothing = false;  // one of these tokens sees nothing
+  Token k{0, 0, 0};
+  for (int t = t_first; t < t_end; ++t) {
+    k = token_of(p, t, false);
+    mine += cost_of(k);
+    nothing |= k.hi == 0;
+  }
   long long to = mine, whole;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -565,37 +645,44 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       whole += scan[w];
     }
   }
-  for (int t = cta; t < p.tokens; t += int(gridDim.x))  // tokens that see nothing
-    if (token_of(p, t, threadIdx.x == 0).hi == 0)
-      for (int e = threadIdx.x; e < p.n_heads * p.head_dim; e += kThreads)
-        reinterpret_cast<AT*>(p.out)[int64_t(t) * p.n_heads * p.head_dim + e] = DT<AT>::from_f32(0.f);
+  if (wide ? __syncthreads_or(nothing) : __any_sync(0xffffffffu, nothing))
+    for (int t = cta; t < p.tokens; t += int(gridDim.x))
+      if (token_of(p, t, threadIdx.x == 0).hi == 0)
+        for (int e = threadIdx.x; e < p.n_heads * p.head_dim; e += kThreads)
+          reinterpret_cast<AT*>(p.out)[int64_t(t) * p.n_heads * p.head_dim + e] = DT<AT>::from_f32(0.f);
   if (whole == 0) return;
-  const TlShares shares = tl_shares(whole * segs, int(gridDim.x), p.least_units, (long long)(p.tokens) * segs);
+  const TlShares shares = tl_shares(whole * segs, int(gridDim.x), kLeastUnits, (long long)(p.tokens) * segs);
   if (cta >= shares.ctas) return;
   const long long begin = tl_share_begin(shares, cta), end = tl_share_begin(shares, cta + 1);
   Cursor c;
   long long into = 0;  // how far the share's begin lies in the units of its token
   const bool found = (to - mine) * segs <= begin && begin < to * segs;  // one thread's
-  c.t = 0;
+  c.t = t_first;
   if (found) {
     into = begin - (to - mine) * segs;
-    for (c.t = t_first; c.t < t_end; ++c.t) {
-      const long long n = (long long)(cost_of(c.t)) * segs;
-      if (into < n) break;
-      into -= n;
-    }
+    if (chunk > 1)
+      for (;; ++c.t) {
+        k = token_of(p, c.t, false);
+        const long long n = (long long)(cost_of(k)) * segs;
+        if (into < n) break;
+        into -= n;
+      }
   }
   if (wide) {
     if (found) { found_token = c.t; found_begin = into; }
     __syncthreads();
     c.t = found_token;
     into = found_begin;
+    c.template open<KEYS>(p);
   } else {
     const int from = __ffs(__ballot_sync(0xffffffffu, found)) - 1;
     c.t = __shfl_sync(0xffffffffu, c.t, from);
     into = __shfl_sync(0xffffffffu, into, from);
+    c.k.lo = __shfl_sync(0xffffffffu, k.lo, from);
+    c.k.hi = __shfl_sync(0xffffffffu, k.hi, from);
+    c.k.seq = __shfl_sync(0xffffffffu, k.seq, from);
+    c.n = tl_tiles(c.k.lo, c.k.hi, KEYS);
   }
-  c.template open<KEYS>(p);
   c.seg = int(tl_quotient(into, c.n + kLead));
   c.head(p);
   long long tile0 = begin - (into - (long long)(c.seg) * (c.n + kLead)) + kLead;  // the unit of the part's first tile
@@ -633,13 +720,13 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       b.key0 = c.template first_key<KEYS>(c.u);
       b.key = b.key0 + (TMA ? lane * KEYS : lane);
       b.page = -1;
-      if (TMA ? lane < b.n : lane < KEYS && b.key >= b.k.lo && b.key < b.k.hi) b.page = __ldg(p.page_table + b.k.seq * p.max_pages + tl_divide(b.key, p.page_div));
+      if (TMA ? lane < b.n : lane < KEYS && b.key >= b.k.lo && b.key < b.k.hi) b.page = __ldg(p.page_table + int64_t(b.k.seq) * p.max_pages + tl_divide(b.key, p.page_div));
       c.u += b.n;
       return b;
     };
     Batch now = look_up();
-    int stage = 0, issued = 0;
-    uint32_t parity = 1;  // of the phase before the first: the ring is empty
+    int stage = 0, lap = 0, issued = 0;
+    const int boxes = 2 * ((p.head_dim * int(sizeof(AT)) + 127) / 128), at_once = min(4, 32 / boxes), my_tile = lane / boxes, my_box = lane % boxes;
     bool ok = true;
     while (now.n > 0 && ok) {
       const Batch then = look_up();
@@ -647,50 +734,55 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       if (wanted && !there) atomicOr(p.status, kBadPage);
       const int in_page = now.key - tl_divide(now.key, p.page_div) * p.page_size;
       const int64_t row = (int64_t(now.page) * p.n_kv_heads + now.kvh) * p.page_size + in_page;
-      for (int j = 0; j < now.n; ++j) {
-        if (!mbar_wait_all(&empty[stage], parity, &abort_flag)) { ok = false; break; }
-        uint8_t* at = sm + stage * kStageBytes<Tile>;
-        if (TMA) {
-          const int key0 = now.key0 + j * KEYS, y = __shfl_sync(0xffffffffu, int(row), j);
-          const bool copied = __shfl_sync(0xffffffffu, int(there), j) != 0;
-          if (lane == 0) {
+      if (TMA) {
+        // Some tiles at once, a lane for each box: a copy costs a warp about 50 ns to issue, whichever lanes do
+        for (int j = 0; j < now.n; j += at_once) {
+          const int n = min(at_once, now.n - j), key0 = now.key0 + (j + my_tile) * KEYS;
+          const int y = __shfl_sync(0xffffffffu, int(row), j + my_tile);
+          const bool mine = my_tile < n, copied = __shfl_sync(0xffffffffu, int(there), j + my_tile) != 0;
+          int to_stage = stage + my_tile, to_lap = lap;
+          if (to_stage >= p.stages) { to_stage -= p.stages; ++to_lap; }
+          // (the first lap: the phase before the first)
+          if (!__all_sync(0xffffffffu, !mine || mbar_wait(&empty[to_stage], (to_lap & 1) ^ 1, &abort_flag))) { ok = false; break; }
+          if (mine && my_box == 0) {
             uint32_t seen = kAll;
             if (key0 < now.k.lo) seen &= kAll << (now.k.lo - key0);
             if (key0 + KEYS > now.k.hi) seen &= kAll >> (key0 + KEYS - now.k.hi);
-            seen_of[stage] = copied ? seen : 0;
-            if (copied) {
-              const int boxes = (p.head_dim * int(sizeof(AT)) + 127) / 128;
-              mbar_expect_tx(&full[stage], uint32_t(2 * boxes * kBoxBytes<Tile>));
-              for (int b = 0; b < boxes; ++b) {
-                tma_load_2d(at + b * kBoxBytes<Tile>, &k_map, b * (128 / int(sizeof(AT))), y, &full[stage]);
-                tma_load_2d(at + kHalf + b * kBoxBytes<Tile>, &v_map, b * (128 / int(sizeof(AT))), y, &full[stage]);
-              }
-            } else {
-              mbar_arrive(&full[stage]);
-            }
+            publish(&seen_of[to_stage], to_lap, copied ? seen : 0);
+            if (copied) mbar_expect_tx(&full[to_stage], uint32_t(boxes * kBoxBytes<Tile>));
+            else mbar_arrive(&full[to_stage]);
           }
-          ++issued;
-        } else {
-          const uint32_t seen = __ballot_sync(0xffffffffu, there);
-          const uint32_t ks = smem_u32(at), vs = ks + kHalf;
-          const int chunks = p.head_dim / kPerChunk;
-          for (int r = 0; r < KEYS; ++r) {
-            const int64_t from = __shfl_sync(0xffffffffu, row, r) * p.head_dim;
-            const int bytes = (seen >> r) & 1 ? 16 : 0;
-            for (int ch = lane; ch < chunks; ch += 32) {
-              const uint32_t to_at = (ch >> 3) * kBoxBytes<Tile> + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-              const int64_t e = bytes ? from + ch * kPerChunk : 0;
-              copy16(ks + to_at, reinterpret_cast<const AT*>(p.k_pages) + e, bytes);
-              copy16(vs + to_at, reinterpret_cast<const AT*>(p.v_pages) + e, bytes);
-            }
+          __syncwarp();
+          if (mine && copied) {
+            const int half = boxes >> 1, b = my_box < half ? my_box : my_box - half;
+            tma_load_2d(sm + to_stage * kStageBytes<Tile> + (my_box < half ? 0 : kHalf) + b * kBoxBytes<Tile>, my_box < half ? &k_map : &v_map,
+                        b * (128 / int(sizeof(AT))), y, &full[to_stage]);
           }
-          copy_arrive(&full[stage]);
-          if (lane == 0) {
-            seen_of[stage] = seen;
-            mbar_arrive(&full[stage]);
+          issued += n;
+          stage += n;
+          if (stage >= p.stages) { stage -= p.stages; ++lap; }
+        }
+      } else {
+        if (!mbar_wait_all(&empty[stage], (lap & 1) ^ 1, &abort_flag)) { ok = false; break; }
+        const uint32_t seen = __ballot_sync(0xffffffffu, there);
+        const uint32_t ks = smem_u32(sm + stage * kStageBytes<Tile>), vs = ks + kHalf;
+        const int chunks = p.head_dim / kPerChunk;
+        for (int r = 0; r < KEYS; ++r) {
+          const int64_t from = __shfl_sync(0xffffffffu, row, r) * p.head_dim;
+          const int bytes = (seen >> r) & 1 ? 16 : 0;
+          for (int ch = lane; ch < chunks; ch += 32) {
+            const uint32_t to_at = (ch >> 3) * kBoxBytes<Tile> + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+            const int64_t e = bytes ? from + ch * kPerChunk : 0;
+            copy16(ks + to_at, reinterpret_cast<const AT*>(p.k_pages) + e, bytes);
+            copy16(vs + to_at, reinterpret_cast<const AT*>(p.v_pages) + e, bytes);
           }
         }
-        if (++stage == p.stages) { stage = 0; parity ^= 1; }
+        copy_arrive(&full[stage]);
+        if (lane == 0) {
+          publish(&seen_of[stage], lap, seen);
+          mbar_arrive(&full[stage]);
+        }
+        if (++stage == p.stages) { stage = 0; ++lap; }
       }
       now = then;
     }
@@ -702,45 +794,54 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     return;
   }
 
-  // ---- the consumers: warp w takes the share's tiles w, w + WARPS, ...
+  // ---- the consumers take the share's tiles in turn; a part of few tiles is one warp's, which then needs nobody else
   float* area = reinterpret_cast<float*>(sm + p.stages * kStageBytes<Tile>);
-  int stage = warp, parity = 0, turn = warp;  // turn: how many of the share's tiles lie before this warp's next, from the part's first in the share
-  while (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
+  constexpr int kSmall = 4;
+  int before = 0, small = 0;  // the share's tiles before this part; parts that were one warp's
   bool ok = true, more = true, met = true;
   Tile tile;
-  while (more) {
-    if (c.u < stop) {
+  for (; more; more = advance()) {
+    const int count = stop - c.u;
+    if (count <= 0) continue;
+    const bool starts = c.u == 0, ends = stop == c.n, alone = starts && ends && c.n <= kSmall;
+    const int first = alone ? 0 : (warp + WARPS - before % WARPS) % WARPS, step = alone ? 1 : WARPS;
+    if (!(alone && small++ % WARPS != warp)) {
       tile.begin(p, c.t, c.kvh, c.tile);
-      const bool starts = c.u == 0, ends = stop == c.n;
-      int i = c.u + turn;
-      for (; i < stop; i += WARPS) {
-        if (ok && !mbar_wait_all(&full[stage], parity, &abort_flag)) {
+      for (int j = first; j < count; j += step) {
+        const int lap = tl_divide(before + j, p.stage_div), stage = before + j - lap * p.stages;
+        uint32_t seen = 0;
+        if (ok && !tile_ready(&seen_of[stage], &full[stage], lap, &abort_flag, seen)) {
           ok = false;
           if (lane == 0) { atomicExch(&abort_flag, 1); atomicExch(p.wait_status, TL_DEV_TIMEOUT_FULL); }
         }
         if (ok) {
-          const uint32_t seen = seen_of[stage], ks = smem_u32(sm + stage * kStageBytes<Tile>);
+          const uint32_t ks = smem_u32(sm + stage * kStageBytes<Tile>);
           if (seen) {
             if (TMA && seen != kAll) {  // values that do not count, whatever they are
-              for (int j = lane; j < KEYS * kBoxes<Tile> * 8; j += 32) {
-                const int r = (j >> 3) % KEYS;
-                if (!((seen >> r) & 1)) reinterpret_cast<uint4*>(sm + stage * kStageBytes<Tile> + kHalf)[j] = make_uint4(0, 0, 0, 0);
+              for (int i = lane; i < KEYS * kBoxes<Tile> * 8; i += 32) {
+                const int r = (i >> 3) % KEYS;
+                if (!((seen >> r) & 1)) reinterpret_cast<uint4*>(sm + stage * kStageBytes<Tile> + kHalf)[i] = make_uint4(0, 0, 0, 0);
               }
               __syncwarp();
             }
-            tile.template take<OPTIONS>(p, ks, ks + kHalf, seen, c.template first_key<KEYS>(i) + 1 - c.k.hi);
+            tile.template take<OPTIONS>(p, ks, ks + kHalf, seen, c.template first_key<KEYS>(c.u + j) + 1 - c.k.hi);
             if (TMA && seen != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty[stage]);
         }
-        stage += WARPS;
-        while (stage >= p.stages) { stage -= p.stages; parity ^= 1; }
       }
-      turn = i - stop;
-
       // The end of this part, or of this CTA's share of it
       const int rows = min(Tile::ROWS, p.rep - c.tile * Tile::ROWS), h0 = c.kvh * p.rep + c.tile * Tile::ROWS;
+      if (alone) {
+        const bool odd = tile.finish(reinterpret_cast<AT*>(p.out) + (int64_t(c.t) * p.n_heads + h0) * p.head_dim, p.head_dim, rows);
+        if (Tile::kRedo && __any_sync(0xffffffffu, odd)) {
+          __syncwarp();
+          for (int i = 0; i < rows * DPAD; i += 32) row_again<AT>(p, c.k, c.k.hi - 1, c.t, h0 + i / DPAD, c.kvh, i % DPAD);
+        }
+        before += count;
+        continue;
+      }
       float *wo = area, *wm = wo + WARPS * rows * kPitch<Tile>, *wl = wm + WARPS * rows;
       if (!met) consumers_meet<Tile>();  // the area is free again
       met = false;
@@ -751,9 +852,10 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
         const int r = e / DPAD, d = e - r * DPAD;
         float v[4] = {o.x, o.y, o.z, o.w};
         bool odd = false;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key's page is there, nothing is seen
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[j] = sum == 0.f ? 0.f : v[j] / sum;  // no key's page is there: nothing is seen
+          v[j] *= inv;
           odd |= !isfinite(v[j]);
         }
         if (d < p.head_dim) {
@@ -802,10 +904,10 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
         }
       }
       if (!(starts && ends)) {
-        // The part's CTAs are first .. first + count - 1.  Whoever comes last of a group of kGroup joins what the group has left, in the place of the
+        // The part's CTAs are head .. head + ctas - 1.  Whoever comes last of a group of kGroup joins what the group has left, in the place of the
         // first of them, and whoever ends the last group joins the groups'.
-        const int first = tl_share_owner(shares, tile0), count = tl_share_owner(shares, tile0 + c.n - 1) - first + 1;
-        const int group = (cta - first) / kGroup, groups = (count + kGroup - 1) / kGroup, members = min(kGroup, count - group * kGroup);
+        const int head = tl_share_owner(shares, tile0), ctas = tl_share_owner(shares, tile0 + c.n - 1) - head + 1;
+        const int group = (cta - head) / kGroup, groups = (ctas + kGroup - 1) / kGroup, members = min(kGroup, ctas - group * kGroup);
         auto last_of = [&](unsigned* arrived, int of) {
           consumers_meet<Tile>();
           if (threadIdx.x == 0) {
@@ -817,20 +919,20 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
           consumers_meet<Tile>();
           return is_last != 0;
         };
-        bool done = last_of(p.arrivals + slot_of(first, group * kGroup), members);
-        if (done) {
-          join<Tile>(p.slots, first, group * kGroup, 1, members, rows, area);
-          if (groups > 1) {
-            float* to_slot = p.slots + int64_t(slot_of(first, group * kGroup)) * slot_floats<Tile>();
+        bool done = true;
+#pragma unroll 1
+        for (int level = 0; done && level < (groups > 1 ? 2 : 1); ++level) {
+          if (level == 1) {
+            float* to_slot = p.slots + int64_t(slot_of(head, group * kGroup)) * slot_floats<Tile>();
             for (int e = threadIdx.x * 4; e < rows * DPAD; e += kConsumers<Tile> * 4)
               __stcg(reinterpret_cast<float4*>(to_slot + e), *reinterpret_cast<const float4*>(area + e));
             if (int(threadIdx.x) < rows) {
               __stcg(to_slot + kSlotMax<Tile> + threadIdx.x, area[rows * DPAD + threadIdx.x]);
               __stcg(to_slot + kSlotSum<Tile> + threadIdx.x, area[rows * DPAD + rows + threadIdx.x]);
             }
-            done = last_of(p.arrivals + 2 * gridDim.x + first, groups);
-            if (done) join<Tile>(p.slots, first, 0, kGroup, groups, rows, area);
           }
+          done = last_of(level == 0 ? p.arrivals + slot_of(head, group * kGroup) : p.arrivals + 2 * gridDim.x + head, level == 0 ? members : groups);
+          if (done) join<Tile>(p.slots, head, level == 0 ? group * kGroup : 0, level == 0 ? 1 : kGroup, level == 0 ? members : groups, rows, area);
         }
         if (done)
           for (int e0 = warp * 128; e0 < rows * DPAD; e0 += WARPS * 128) {
@@ -840,15 +942,16 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
           }
       }
     }
-    more = advance();
+    before += count;
   }
 }
 
 template <class Tile, bool OPTIONS, bool TMA>
 cudaError_t launch(tl_ctx* ctx, PagedArgs& p, const CUtensorMap& k_map, const CUtensorMap& v_map, int64_t most_units) {
   // Shared memory in equal parts for the resident CTAs (1 KB of each is the system's, the barriers take less than another)
-  const int rows = std::min(Tile::ROWS, p.rep), room = (228 / Tile::CTAS - 2) * 1024 - area_bytes<Tile>(rows);
+  const int rows = std::min(Tile::ROWS, p.rep), room = (228 / Tile::CTAS - 1) * 1024 - 2048 - area_bytes<Tile>(rows);
   p.stages = std::min(kMaxStages, room / kStageBytes<Tile>);
+  p.stage_div = tl_divide_by(p.stages);
   const int smem = p.stages * kStageBytes<Tile> + area_bytes<Tile>(rows);
   auto kernel = paged_attention_kernel<Tile, OPTIONS, TMA>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -895,7 +998,8 @@ cudaError_t launch_f32(tl_ctx* ctx, PagedArgs& p, int64_t longest) {
 }
 
 // Parts of tokens for two CTAs an SM of the largest slot, and the arrivals: one size for all calls, so that no captured call's scratch is replaced.
-constexpr int kSlotFloats = 16 * 130, kLeastUnits = 24;
+constexpr int kSlotFloats = 16 * 130;
+static_assert(kMaxStages <= 32 + 32 * kConsumerWarps, "a barrier a thread");
 static_assert(slot_floats<MmaTile<__half, 64, 2>>() <= kSlotFloats && slot_floats<F32Tile<256, 4>>() <= kSlotFloats && slot_floats<F32Tile<128, 8>>() <= kSlotFloats, "slots");
 static_assert(slot_floats<MmaTile<__half, 256, 1>>() <= kSlotFloats && slot_floats<MmaTile<__half, 128, 2>>() <= kSlotFloats, "slots");
 int32_t secure_scratch(tl_ctx* ctx) {
@@ -948,7 +1052,7 @@ int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32
   p.qt = q_token_stride; p.qh = q_head_stride; p.n_pages = cache->n_pages;
   p.tokens = int32_t(tokens); p.n_heads = int32_t(n_heads); p.n_kv_heads = cache->n_kv_heads; p.rep = int32_t(n_heads / cache->n_kv_heads);
   p.head_dim = cache->head_dim; p.page_size = cache->page_size; p.n_seqs = cache->n_seqs; p.max_pages = cache->max_pages;
-  p.window = window; p.scale = scale; p.softcap = softcap; p.cap_exp = softcap > 0.f ? 2.f * kLog2e / softcap : 0.f; p.least_units = kLeastUnits;
+  p.window = window; p.scale = scale; p.softcap = softcap; p.cap_exp = softcap > 0.f ? 2.f * kLog2e / softcap : 0.f;
   p.page_div = tl_divide_by(cache->page_size);
   p.status = ctx->dev_status + 1;
   p.wait_status = ctx->dev_status;
