@@ -175,7 +175,7 @@ def test_every_unit_has_one_owner(stub):
                                         ([1], 296), ([1, 1], 296), ([2000] + [1] * 100, 148)])
 def test_parts_meet_in_slots_of_their_own(stub, tiles, most):
     """The shares walked on the host as the kernel walks them: every tile is taken once, the CTAs that have tiles of a part are those between the owners of its first and
-    last, each leaves what it made of a part in a slot that no other part uses, and no two groups of twelve count their arrivals in one place."""
+    last, each leaves what it made of a part in a slot that no other part uses, and no two groups of thirteen count their arrivals in one place."""
     lead = stub.stub_lead()
     starts_at = list(itertools.accumulate([0] + [lead + n for n in tiles]))
     args = starts_at[-1], most, 24, len(tiles)
@@ -197,7 +197,7 @@ def test_parts_meet_in_slots_of_their_own(stub, tiles, most):
                 slot = 2 * cta + (u == 0)
                 assert slot not in slots
                 slots.add(slot)
-                if (cta - first) % 12 == 0:
+                if (cta - first) % 13 == 0:
                     place = 2 * cta + (cta == first)
                     assert place not in places and place < 2 * most
                     places.add(place)

@@ -9,7 +9,7 @@
 // depends on a length, so that a captured call serves sequences that grow.  A producer warp looks up the pages, a batch of tiles ahead, and fills a ring of tiles
 // in shared memory across the borders of tokens and heads; four consumer warps take the tiles in turn, each with a softmax of its own, and
 // meet at the end of a token's keys.  Where a share ends inside a token's keys the CTA leaves maximum, sum and output in scratch, and whoever of that
-// token's CTAs comes last joins them in the order of the keys (in groups of 12 first, where they are many), so that no result depends on timing.
+// token's CTAs comes last joins them in the order of the keys (in groups of 13 first, where they are many), so that no result depends on timing.
 //
 // The ring.  Where a tile's rows are neighbours in a page (page_size a multiple of the tile), TMA boxes of 128-byte columns, 128-byte swizzle: an
 // instruction for each 2 KB.  Other page sizes: cp.async into the same layout, 16 bytes a lane.
@@ -36,7 +36,7 @@ namespace {
 #define PA_CTAS 2
 #define PA_WARPS 3
 #endif
-constexpr int kCtas = PA_CTAS, kConsumerWarps = PA_WARPS, kGroup = 12, kMaxStages = 48, kLeastUnits = 12;
+constexpr int kCtas = PA_CTAS, kConsumerWarps = PA_WARPS, kGroup = 13, kMaxStages = 48, kLeastUnits = 12;
 
 struct PagedArgs {
   const void *q, *k_pages, *v_pages;
@@ -195,7 +195,8 @@ struct MmaTile {
   uint32_t q[NT][DPAD / 16][2];
   float o[NT][DPAD / 16][4], m[NT][2], l[NT][2], slope[NT][2];
 
-  __device__ __forceinline__ void begin(const PagedArgs& p, int t, int kvh, int tile) {
+  // The queries of a part, which may still be on their way while the one before it ends
+  __device__ __forceinline__ void load(const PagedArgs& p, int t, int kvh, int tile) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -208,10 +209,18 @@ struct MmaTile {
           q[nt][i][j] = row < p.rep && 16 * i + 8 * j < p.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * i + 8 * j)) : 0u;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[nt][e] = -INFINITY;
-        l[nt][e] = 0.f;
         const int r = tile * ROWS + nt * 8 + 2 * c + e;
         slope[nt][e] = p.slopes && r < p.rep ? p.slopes[kvh * p.rep + r] * kLog2e : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[nt][e] = -INFINITY;
+        l[nt][e] = 0.f;
       }
 #pragma unroll
       for (int i = 0; i < DPAD / 16; ++i)
@@ -388,28 +397,34 @@ struct F32Tile {
   float q[ROWS][E], o[ROWS][E];
   float m[kSets], l[kSets], slope[kSets];  // of the row whose score this lane ends up with: its maximum, and the sum over this lane's keys
 
-  __device__ __forceinline__ void begin(const PagedArgs& p, int t, int kvh, int tile) {
+  __device__ __forceinline__ void load(const PagedArgs& p, int t, int kvh, int tile) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int row = tile * ROWS + r;
       const float* qp = reinterpret_cast<const float*>(p.q) + int64_t(t) * p.qt + int64_t(kvh * p.rep + row) * p.qh + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        q[r][e] = row < p.rep && lane * E + e < p.head_dim ? __ldg(qp + e) : 0.f;
-        o[r][e] = 0.f;
-      }
+      for (int e = 0; e < E; ++e) q[r][e] = row < p.rep && lane * E + e < p.head_dim ? __ldg(qp + e) : 0.f;
     }
 #pragma unroll
     for (int s = 0; s < kSets; ++s) {
-      m[s] = -INFINITY;
-      l[s] = 0.f;
       const int row = tile * ROWS + s * kRowsOfSet + (lane >> (5 - kLog)) / KEYS;
       slope[s] = p.slopes && row < p.rep ? p.slopes[kvh * p.rep + row] * kLog2e : 0.f;
     }
   }
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[r][e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) {
+      m[s] = -INFINITY;
+      l[s] = 0.f;
+    }
+  }
   // this lane's dimensions of row r
-  static __device__ __forceinline__ void load(uint32_t tile_at, int r, float (&v)[E]) {
+  static __device__ __forceinline__ void row_of(uint32_t tile_at, int r, float (&v)[E]) {
     const int lane = threadIdx.x & 31;
     if (E == 2) {
       const int c = lane >> 1;
@@ -430,7 +445,7 @@ struct F32Tile {
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
       float k[E];
-      load(ks, j, k);
+      row_of(ks, j, k);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         float x = 0.f;
@@ -473,7 +488,7 @@ struct F32Tile {
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
       float v[E];
-      load(vs, j, v);
+      row_of(vs, j, v);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         const float w = __shfl_sync(0xffffffffu, pr[r / kRowsOfSet], ((r % kRowsOfSet) * KEYS + j) << (5 - kLog));
@@ -534,20 +549,25 @@ template <class Tile> constexpr int kSlotSum = kSlotMax<Tile> + Tile::ROWS;
 
 // The slot in which CTA first + i of a token's CTAs leaves its part: the first of them starts the token, the others have it begun elsewhere.
 __device__ __forceinline__ int slot_of(int first, int i) { return 2 * (first + i) + (i == 0 ? 1 : 0); }
-// Parts i = from, from + step, ... of a token, `count` of them (at most 32), become one in area: [rows][DPAD] outputs, [rows] maxima, [rows] sums, and
-// then the [rows][count] factors used.  The consumer warps call it.
-template <class Tile> __device__ void join(const float* slots, int first, int from, int step, int count, int rows, float* area) {
-  float *maxima = area + rows * Tile::DPAD, *sums = maxima + rows, *factor = sums + rows;
+// Parts i = from, from + step, ... of a token, `count` of them (at most 32), by all threads of the CTA: write(e, output, maximum, sum) gets four
+// neighbouring values of [rows][DPAD] from e on, not yet divided by the sum.  The loads of kGroup of them are on their way together.  area: rows * 34 floats.
+template <class Tile, typename W> __device__ __forceinline__ void join(const float* slots, int first, int from, int step, int count, int rows, float* area, W&& write) {
+  constexpr int kThreads = 32 + kConsumers<Tile>, kItems = (Tile::ROWS * Tile::DPAD / 4 + kThreads - 1) / kThreads, kTogether = kItems > 2 ? 2 : kItems;
+  float *maxima = area, *sums = maxima + rows, *factor = sums + rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto part = [&](int i) { return slots + int64_t(slot_of(first, from + min(i, count - 1) * step)) * slot_floats<Tile>(); };
-  // the first outputs are on their way while the factors are worked out
-  constexpr int kLoads = 12;
-  const int e_first = threadIdx.x * 4;
-  float4 v[kLoads];
+  auto part = [&](int i) { return slots + int64_t(slot_of(first, from + i * step)) * slot_floats<Tile>(); };
+  float4 v[kTogether][kGroup];
+  auto fetch = [&](int e0, int i0) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i)
-    if (e_first < rows * Tile::DPAD) v[i] = __ldcg(reinterpret_cast<const float4*>(part(i) + e_first));
-  for (int r = warp; r < rows; r += Tile::WARPS) {
+    for (int k = 0; k < kTogether; ++k)
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const int e = e0 + 4 * (k * kThreads + int(threadIdx.x));
+        if (i0 + i < count && e < rows * Tile::DPAD) v[k][i] = __ldcg(reinterpret_cast<const float4*>(part(i0 + i) + e));
+      }
+  };
+  fetch(0, 0);
+  for (int r = warp; r < rows; r += kThreads / 32) {
     float mx = -INFINITY, sum = 0.f;
     if (lane < count) { mx = __ldcg(part(lane) + kSlotMax<Tile> + r); sum = __ldcg(part(lane) + kSlotSum<Tile> + r); }
     float top = mx;
@@ -557,28 +577,44 @@ template <class Tile> __device__ void join(const float* slots, int first, int fr
     sum *= f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane < count) factor[r * count + lane] = f;
+    if (lane < count) factor[r * 32 + lane] = f;
     if (lane == 0) { maxima[r] = top; sums[r] = sum; }
   }
-  consumers_meet<Tile>();
-  for (int e = e_first; e < rows * Tile::DPAD; e += kConsumers<Tile> * 4) {
-    const int r = e / Tile::DPAD;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncthreads();
 #pragma unroll 1
-    for (int i0 = 0; i0 < count; i0 += kLoads) {
-      if (i0 > 0 || e != e_first)
+  for (int e0 = 0; e0 < rows * Tile::DPAD; e0 += 4 * kTogether * kThreads) {
+    float4 a[kTogether];
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(part(i0 + i) + e));
+    for (int k = 0; k < kTogether; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += kGroup) {
+      if (e0 + i0 > 0) fetch(e0, i0);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        if (i0 + i < count) {
-          const float f = factor[r * count + i0 + i];
-          a.x = fmaf(f, v[i].x, a.x); a.y = fmaf(f, v[i].y, a.y); a.z = fmaf(f, v[i].z, a.z); a.w = fmaf(f, v[i].w, a.w);
-        }
+      for (int k = 0; k < kTogether; ++k) {
+        const int r = min((e0 + 4 * (k * kThreads + int(threadIdx.x))) / Tile::DPAD, rows - 1);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i)
+          if (i0 + i < count) {
+            const float f = factor[r * 32 + i0 + i];
+            a[k].x = fmaf(f, v[k][i].x, a[k].x); a[k].y = fmaf(f, v[k][i].y, a[k].y);
+            a[k].z = fmaf(f, v[k][i].z, a[k].z); a[k].w = fmaf(f, v[k][i].w, a[k].w);
+          }
+      }
     }
-    *reinterpret_cast<float4*>(area + e) = a;
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) {
+      const int e = e0 + 4 * (k * kThreads + int(threadIdx.x)), r = min(e / Tile::DPAD, rows - 1);
+      write(e, a[k], maxima[r], sums[r]);  // by whole warps; e may lie past the end
+    }
   }
-  consumers_meet<Tile>();
+}
+// What the CTAs of a part have left in their slots before this is seen by the one that comes last
+__device__ __forceinline__ bool arrive(unsigned* at, int of) {
+  unsigned old;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(at) : "memory");
+  if (old != unsigned(of) - 1) return false;
+  *at = 0;  // for the next launch
+  return true;
 }
 
 template <class Tile, bool OPTIONS, bool TMA>
@@ -589,10 +625,17 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
   constexpr int kHalf = kStageBytes<Tile> / 2, kPerChunk = 16 / int(sizeof(AT));
   constexpr uint32_t kAll = (1u << KEYS) - 1;
   extern __shared__ __align__(1024) uint8_t sm[];
+  struct Part {
+    int t, kvh, tile, n;
+    Token k;
+    long long tile0;
+    int left;  // in a slot: other CTAs have tiles of it too
+  };
+  __shared__ Part cut[2];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
   __shared__ uint32_t seen_of[kMaxStages];
   __shared__ long long found_begin, scan[kThreads / 32];
-  __shared__ int found_token, is_last, abort_flag;
+  __shared__ int found_token, is_last[2], groups_done, abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = int(blockIdx.x);
   if (int(threadIdx.x) < p.stages) {
     mbar_init(&full[threadIdx.x], TMA ? 1 : 33);  // cp.async: every lane's copies, and the word of what is seen
@@ -601,7 +644,7 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     mbar_fence_init();
   }
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    abort_flag = is_last[0] = is_last[1] = cut[0].left = cut[1].left = 0;
     if (TMA) { tma_prefetch_desc(&k_map); tma_prefetch_desc(&v_map); }
   }
   if (p.head_dim < DPAD) {  // no copy writes the padding: it is zero from here on
@@ -791,55 +834,97 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       if (TMA && lane == 0) tma_drain(full, p.stages, issued);
       if (!TMA) asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    return;
   }
 
   // ---- the consumers take the share's tiles in turn; a part of few tiles is one warp's, which then needs nobody else
-  float* area = reinterpret_cast<float*>(sm + p.stages * kStageBytes<Tile>);
   constexpr int kSmall = 4;
-  int before = 0, small = 0;  // the share's tiles before this part; parts that were one warp's
-  bool ok = true, more = true, met = true;
-  Tile tile;
-  for (; more; more = advance()) {
-    const int count = stop - c.u;
-    if (count <= 0) continue;
-    const bool starts = c.u == 0, ends = stop == c.n, alone = starts && ends && c.n <= kSmall;
-    const int first = alone ? 0 : (warp + WARPS - before % WARPS) % WARPS, step = alone ? 1 : WARPS;
-    if (!(alone && small++ % WARPS != warp)) {
-      tile.begin(p, c.t, c.kvh, c.tile);
-      for (int j = first; j < count; j += step) {
-        const int lap = tl_divide(before + j, p.stage_div), stage = before + j - lap * p.stages;
-        uint32_t seen = 0;
-        if (ok && !tile_ready(&seen_of[stage], &full[stage], lap, &abort_flag, seen)) {
-          ok = false;
-          if (lane == 0) { atomicExch(&abort_flag, 1); atomicExch(p.wait_status, TL_DEV_TIMEOUT_FULL); }
-        }
-        if (ok) {
-          const uint32_t ks = smem_u32(sm + stage * kStageBytes<Tile>);
-          if (seen) {
-            if (TMA && seen != kAll) {  // values that do not count, whatever they are
-              for (int i = lane; i < KEYS * kBoxes<Tile> * 8; i += 32) {
-                const int r = (i >> 3) % KEYS;
-                if (!((seen >> r) & 1)) reinterpret_cast<uint4*>(sm + stage * kStageBytes<Tile> + kHalf)[i] = make_uint4(0, 0, 0, 0);
-              }
-              __syncwarp();
-            }
-            tile.template take<OPTIONS>(p, ks, ks + kHalf, seen, c.template first_key<KEYS>(c.u + j) + 1 - c.k.hi);
-            if (TMA && seen != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  float* area = reinterpret_cast<float*>(sm + p.stages * kStageBytes<Tile>);
+  // Four neighbouring values of a row by each thread
+  auto store = [&](const Part& w, int h0, int e, float4 o, float sum) {
+    const int r = e / DPAD, d = e - r * DPAD;
+    float v[4] = {o.x, o.y, o.z, o.w};
+    bool odd = false;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key's page is there, nothing is seen
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] *= inv;
+      odd |= !isfinite(v[j]);
+    }
+    if (d < p.head_dim) {
+      AT* to_at = reinterpret_cast<AT*>(p.out) + (int64_t(w.t) * p.n_heads + h0 + r) * p.head_dim + d;
+      if (sizeof(AT) == 4) {
+        *reinterpret_cast<float4*>(to_at) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        AT h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = DT<AT>::from_f32(v[j]);
+        *reinterpret_cast<uint2*>(to_at) = *reinterpret_cast<const uint2*>(h);
+      }
+    }
+    return Tile::kRedo && odd && d < p.head_dim;
+  };
+  // After the stores of a warp's 128 values from e0 on: the rows' blocks of 32 that have one that is not finite, again
+  auto store_again = [&](const Part& w, int h0, uint32_t odd, int e0) {
+    if (!odd) return;
+    __syncwarp();
+    for (int b = 0; b < 4; ++b)
+      if ((odd >> (8 * b)) & 0xff) row_again<AT>(p, w.k, w.k.hi - 1, w.t, h0 + (e0 + 32 * b) / DPAD, w.kvh, (e0 + 32 * b) % DPAD);
+  };
+  if (warp < WARPS) {
+    int before = 0, small = 0;  // the share's tiles before this part; parts that were one warp's
+    bool ok = true, met = true;
+    auto settle = [&](bool more) {
+      while (more && c.u >= stop) more = advance();
+      return more;
+    };
+    Tile tile;
+    bool more = settle(true);
+    if (more) tile.load(p, c.t, c.kvh, c.tile);
+    while (more) {
+      const int u = c.u, count = stop - u;
+      const bool starts = u == 0, ends = stop == c.n, alone = starts && ends && c.n <= kSmall, mine = !alone || small++ % WARPS == warp;
+      const Part part{c.t, c.kvh, c.tile, c.n, c.k, tile0, !(starts && ends)};
+      const int rows = min(Tile::ROWS, p.rep - part.tile * Tile::ROWS), h0 = part.kvh * p.rep + part.tile * Tile::ROWS;
+      if (mine) {
+        tile.reset();
+        for (int j = alone ? 0 : (warp + WARPS - before % WARPS) % WARPS; j < count; j += alone ? 1 : WARPS) {
+          const int lap = tl_divide(before + j, p.stage_div), stage = before + j - lap * p.stages;
+          uint32_t seen = 0;
+          if (ok && !tile_ready(&seen_of[stage], &full[stage], lap, &abort_flag, seen)) {
+            ok = false;
+            if (lane == 0) { atomicExch(&abort_flag, 1); atomicExch(p.wait_status, TL_DEV_TIMEOUT_FULL); }
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&empty[stage]);
+          if (ok) {
+            const uint32_t ks = smem_u32(sm + stage * kStageBytes<Tile>);
+            if (seen) {
+              if (TMA && seen != kAll) {  // values that do not count, whatever they are
+                for (int i = lane; i < KEYS * kBoxes<Tile> * 8; i += 32) {
+                  const int r = (i >> 3) % KEYS;
+                  if (!((seen >> r) & 1)) reinterpret_cast<uint4*>(sm + stage * kStageBytes<Tile> + kHalf)[i] = make_uint4(0, 0, 0, 0);
+                }
+                __syncwarp();
+              }
+              tile.template take<OPTIONS>(p, ks, ks + kHalf, seen, c.template first_key<KEYS>(u + j) + 1 - part.k.hi);
+              if (TMA && seen != kAll) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[stage]);
+          }
         }
       }
-      // The end of this part, or of this CTA's share of it
-      const int rows = min(Tile::ROWS, p.rep - c.tile * Tile::ROWS), h0 = c.kvh * p.rep + c.tile * Tile::ROWS;
+      before += count;
+      more = settle(advance());
+      if (more) tile.load(p, c.t, c.kvh, c.tile);
+
+      // The end of the part, or of this CTA's share of it
       if (alone) {
-        const bool odd = tile.finish(reinterpret_cast<AT*>(p.out) + (int64_t(c.t) * p.n_heads + h0) * p.head_dim, p.head_dim, rows);
-        if (Tile::kRedo && __any_sync(0xffffffffu, odd)) {
-          __syncwarp();
-          for (int i = 0; i < rows * DPAD; i += 32) row_again<AT>(p, c.k, c.k.hi - 1, c.t, h0 + i / DPAD, c.kvh, i % DPAD);
+        if (mine) {
+          const bool odd = tile.finish(reinterpret_cast<AT*>(p.out) + (int64_t(part.t) * p.n_heads + h0) * p.head_dim, p.head_dim, rows);
+          if (Tile::kRedo && __any_sync(0xffffffffu, odd)) {
+            __syncwarp();
+            for (int i = 0; i < rows * DPAD; i += 32) row_again<AT>(p, part.k, part.k.hi - 1, part.t, h0 + i / DPAD, part.kvh, i % DPAD);
+          }
         }
-        before += count;
         continue;
       }
       float *wo = area, *wm = wo + WARPS * rows * kPitch<Tile>, *wl = wm + WARPS * rows;
@@ -847,37 +932,6 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       met = false;
       tile.end(wm + warp * rows, wl + warp * rows, wo + warp * rows * kPitch<Tile>, kPitch<Tile>, rows);
       consumers_meet<Tile>();
-      // Four neighbouring values of a row by each thread
-      auto store = [&](int e, float4 o, float sum) {
-        const int r = e / DPAD, d = e - r * DPAD;
-        float v[4] = {o.x, o.y, o.z, o.w};
-        bool odd = false;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key's page is there, nothing is seen
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] *= inv;
-          odd |= !isfinite(v[j]);
-        }
-        if (d < p.head_dim) {
-          AT* to_at = reinterpret_cast<AT*>(p.out) + (int64_t(c.t) * p.n_heads + h0 + r) * p.head_dim + d;
-          if (sizeof(AT) == 4) {
-            *reinterpret_cast<float4*>(to_at) = make_float4(v[0], v[1], v[2], v[3]);
-          } else {
-            AT h[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = DT<AT>::from_f32(v[j]);
-            *reinterpret_cast<uint2*>(to_at) = *reinterpret_cast<const uint2*>(h);
-          }
-        }
-        return Tile::kRedo && odd && d < p.head_dim;
-      };
-      // After the stores of a warp's 128 values from e0 on: the rows' blocks of 32 that have one that is not finite, again
-      auto store_again = [&](uint32_t odd, int e0) {
-        if (!odd) return;
-        __syncwarp();
-        for (int b = 0; b < 4; ++b)
-          if ((odd >> (8 * b)) & 0xff) row_again<AT>(p, c.k, c.k.hi - 1, c.t, h0 + (e0 + 32 * b) / DPAD, c.kvh, (e0 + 32 * b) % DPAD);
-      };
       float* slot = p.slots + int64_t(2 * cta + (starts ? 1 : 0)) * slot_floats<Tile>();
       for (int e0 = warp * 128; e0 < rows * DPAD; e0 += WARPS * 128) {
         const int e = e0 + 4 * lane, r = min(e, rows * DPAD - 1) / DPAD, d = e - r * DPAD;
@@ -895,54 +949,69 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
             o.x = fmaf(w.x, g, o.x); o.y = fmaf(w.y, g, o.y); o.z = fmaf(w.z, g, o.z); o.w = fmaf(w.w, g, o.w);
           }
         }
-        if (starts && ends) {
-          const bool odd = here && store(e, o, sum);
-          store_again(__ballot_sync(0xffffffffu, odd), e0);
+        if (!part.left) {
+          const bool odd = here && store(part, h0, e, o, sum);
+          store_again(part, h0, __ballot_sync(0xffffffffu, odd), e0);
         } else if (here) {
           if (d == 0) { __stcg(slot + kSlotMax<Tile> + r, top); __stcg(slot + kSlotSum<Tile> + r, sum); }
           __stcg(reinterpret_cast<float4*>(slot + e), o);
         }
       }
-      if (!(starts && ends)) {
-        // The part's CTAs are head .. head + ctas - 1.  Whoever comes last of a group of kGroup joins what the group has left, in the place of the
-        // first of them, and whoever ends the last group joins the groups'.
-        const int head = tl_share_owner(shares, tile0), ctas = tl_share_owner(shares, tile0 + c.n - 1) - head + 1;
-        const int group = (cta - head) / kGroup, groups = (ctas + kGroup - 1) / kGroup, members = min(kGroup, ctas - group * kGroup);
-        auto last_of = [&](unsigned* arrived, int of) {
-          consumers_meet<Tile>();
-          if (threadIdx.x == 0) {
-            __threadfence();
-            is_last = atomicAdd(arrived, 1u) == unsigned(of) - 1;
-            if (is_last) *arrived = 0;  // for the next launch
-            __threadfence();
-          }
-          consumers_meet<Tile>();
-          return is_last != 0;
-        };
-        bool done = true;
-#pragma unroll 1
-        for (int level = 0; done && level < (groups > 1 ? 2 : 1); ++level) {
-          if (level == 1) {
-            float* to_slot = p.slots + int64_t(slot_of(head, group * kGroup)) * slot_floats<Tile>();
-            for (int e = threadIdx.x * 4; e < rows * DPAD; e += kConsumers<Tile> * 4)
-              __stcg(reinterpret_cast<float4*>(to_slot + e), *reinterpret_cast<const float4*>(area + e));
-            if (int(threadIdx.x) < rows) {
-              __stcg(to_slot + kSlotMax<Tile> + threadIdx.x, area[rows * DPAD + threadIdx.x]);
-              __stcg(to_slot + kSlotSum<Tile> + threadIdx.x, area[rows * DPAD + rows + threadIdx.x]);
-            }
-          }
-          done = last_of(level == 0 ? p.arrivals + slot_of(head, group * kGroup) : p.arrivals + 2 * gridDim.x + head, level == 0 ? members : groups);
-          if (done) join<Tile>(p.slots, head, level == 0 ? group * kGroup : 0, level == 0 ? 1 : kGroup, level == 0 ? members : groups, rows, area);
-        }
-        if (done)
-          for (int e0 = warp * 128; e0 < rows * DPAD; e0 += WARPS * 128) {
-            const int e = e0 + 4 * lane;
-            const bool odd = e < rows * DPAD && store(e, *reinterpret_cast<const float4*>(area + e), area[rows * DPAD + rows + e / DPAD]);
-            store_again(__ballot_sync(0xffffffffu, odd), e0);
-          }
-      }
+      if (part.left && threadIdx.x == 0) cut[starts ? 1 : 0] = part;
     }
-    before += count;
+  }
+
+  // What others have tiles of too: at most the part that the share's begin cuts and the one that its end cuts.  Only now: a fence and an atomic take microseconds
+  // while the copies are at full rate, and the next part's tiles would wait behind them (8 x 8 x 4000 keys: CTAs with a cut inside their share
+  // ended 5 to 9 us after the others).  A part's CTAs are head .. head + ctas - 1; whoever comes last of a group of kGroup joins what the group
+  // has left, in the place of the first of them, and whoever ends the last group joins the groups'.
+  __syncthreads();
+  struct Crowd {
+    int head, group, groups, members;
+  };
+  auto crowd_of = [&](const Part& w) {
+    Crowd g;
+    g.head = tl_share_owner(shares, w.tile0);
+    const int ctas = tl_share_owner(shares, w.tile0 + w.n - 1) - g.head + 1;
+    g.group = (cta - g.head) / kGroup;
+    g.groups = (ctas + kGroup - 1) / kGroup;
+    g.members = min(kGroup, ctas - g.group * kGroup);
+    return g;
+  };
+  if (threadIdx.x < 2 && cut[threadIdx.x].left) {
+    const Crowd g = crowd_of(cut[threadIdx.x]);
+    is_last[threadIdx.x] = arrive(p.arrivals + slot_of(g.head, g.group * kGroup), g.members);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if (!is_last[i]) continue;
+    const Part w = cut[i];
+    const Crowd g = crowd_of(w);
+    const int rows = min(Tile::ROWS, p.rep - w.tile * Tile::ROWS), h0 = w.kvh * p.rep + w.tile * Tile::ROWS;
+    bool whole_part = g.groups == 1;
+#pragma unroll 1
+    for (int level = 0; level < 2; ++level) {
+      float* to_slot = p.slots + int64_t(slot_of(g.head, g.group * kGroup)) * slot_floats<Tile>();
+      __syncthreads();  // the area is free
+      join<Tile>(p.slots, g.head, level == 0 ? g.group * kGroup : 0, level == 0 ? 1 : kGroup, level == 0 ? g.members : g.groups, rows, area,
+                 [&](int e, float4 o, float top, float sum) {
+                   const bool here = e < rows * DPAD;
+                   if (whole_part) {
+                     const bool odd = here && store(w, h0, e, o, sum);
+                     store_again(w, h0, __ballot_sync(0xffffffffu, odd), e - 4 * lane);
+                   } else if (here) {
+                     __stcg(reinterpret_cast<float4*>(to_slot + e), o);
+                     if (e % DPAD == 0) { __stcg(to_slot + kSlotMax<Tile> + e / DPAD, top); __stcg(to_slot + kSlotSum<Tile> + e / DPAD, sum); }
+                   }
+                 });
+      if (whole_part) break;
+      __syncthreads();
+      if (threadIdx.x == 0) groups_done = arrive(p.arrivals + 2 * gridDim.x + g.head, g.groups);
+      __syncthreads();
+      if (!groups_done) break;
+      whole_part = true;
+    }
   }
 }
 
@@ -999,6 +1068,7 @@ cudaError_t launch_f32(tl_ctx* ctx, PagedArgs& p, int64_t longest) {
 
 // Parts of tokens for two CTAs an SM of the largest slot, and the arrivals: one size for all calls, so that no captured call's scratch is replaced.
 constexpr int kSlotFloats = 16 * 130;
+static_assert(kGroup * 32 >= 160 * kCtas, "two levels are enough for so many SMs");
 static_assert(kMaxStages <= 32 + 32 * kConsumerWarps, "a barrier a thread");
 static_assert(slot_floats<MmaTile<__half, 64, 2>>() <= kSlotFloats && slot_floats<F32Tile<256, 4>>() <= kSlotFloats && slot_floats<F32Tile<128, 8>>() <= kSlotFloats, "slots");
 static_assert(slot_floats<MmaTile<__half, 256, 1>>() <= kSlotFloats && slot_floats<MmaTile<__half, 128, 2>>() <= kSlotFloats, "slots");
