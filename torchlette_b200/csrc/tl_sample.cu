@@ -8,7 +8,17 @@
 // over CTAs changes a token, and a border is where it is in 64-bit arithmetic.
 //
 // A cluster of CTAs owns a row, each a contiguous slice; what the CTAs tell each other goes through distributed shared memory.  No scratch, no
-// second launch.
+// second launch.  Bound: HBM for the first pass over a row, L2 and the cluster's meetings after it.
+//
+//   one pass    the row's maximum, and the maxima of 256 groups of its elements.
+//   top-k       up to kMaxQuick: the k-th largest of the group maxima is no more than the k-th largest logit, and little is between them (k = 50: about 55
+//               candidates).  A second pass sends what is not below it to the first CTA, which ranks the candidates by counting and draws.
+//   the rest    a set of kept tokens is narrowed by 2048 bins of counts or masses, linear in the logit, and the bin that holds the border
+//               is resolved by ranking its tokens; where ties or a spread over all magnitudes leave too many in it, by bins of the keys down to one key.
+//               Then a pass over the masses, and the CTA that holds the answer walks its slice.
+//
+// exp in 64 bits by a table of 2^(j/128) and a polynomial on what is left (Tang's table-driven method, 1989): ten operations where the library's exp takes
+// about three times as many.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -21,7 +31,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kBins = 2048;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 16, kBins = 2048, kGroups = 256, kMaxQuick = 192, kCandidates = 1024;
 constexpr uint32_t kNone = 0x007fffffu;  // key of -infinity: never kept
 
 struct SampleArgs {
@@ -33,14 +43,17 @@ struct SampleArgs {
   int32_t vocab, per_cta, shift, vec;  // per_cta: elements of a slice, a multiple of 8; vec: rows start on 16 bytes
 };
 
+using u64 = unsigned long long;
 struct Shared {
-  unsigned long long warp_max[kMaxCluster * kWarps];  // (key, ~index) of every warp of the cluster
-  unsigned long long told[2][kMaxCluster];            // one value a CTA, two turns
-  unsigned long long mass[kBins];
-  unsigned long long part[kWarps];
-  uint32_t count[kBins];
-  uint32_t low, high, bin, bin_count, token;
-  unsigned long long above;
+  u64 group_max[kGroups];      // (key, ~index) of every group of the cluster
+  u64 told[2][kMaxCluster];    // one value a CTA, two turns
+  u64 part[kWarps];
+  double table[128];           // 2^(j / 128)
+  uint32_t count[kBins], mass_low[kBins], mass_high[kBins];  // of this CTA's slice
+  u64 cand[kCandidates];       // in the first CTA: (key, ~index)
+  u64 sorted[kCandidates], weight[kCandidates];
+  uint32_t n_cand, low, high, bin, bin_count, token, border_key, border_index;
+  u64 above;
 };
 
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -54,10 +67,11 @@ __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x 
 // A row's view of one CTA: its slice, the tokens kept so far, and the cluster around it.
 template <typename T> struct Row {
   const T* x;
-  int begin, end, rank, ctas, turn;
+  int begin, end, rank_in, ctas, turn;
   bool vec;
   float max;
-  double inv_t, one;
+  double scale, offset, lowest;  // 128 log2 of a weight is logit * scale + offset; below lowest nothing is left
+  int shift;
   uint32_t threshold, min_key;  // kept: key > threshold, or equal and index <= last; and key >= min_key once min-p counts
   int last;
   Shared* s;
@@ -84,12 +98,20 @@ template <typename T> struct Row {
     for (int i = begin + int(threadIdx.x) * 8; i < end; i += kThreads * 8) each_of(i, f);
   }
   __device__ __forceinline__ bool kept(int i, uint32_t key) const { return key > threshold || (key == threshold && i <= last); }
-  __device__ __forceinline__ unsigned long long mass_of(float v) const {
-    if (v == max) return static_cast<unsigned long long>(one);
-    const double d = double(v) - double(max);
-    return d == -INFINITY ? 0ull : static_cast<unsigned long long>(__double2ll_rn(exp(d * inv_t) * one));
+  __device__ __forceinline__ u64 mass_of(float v) const {
+    if (v == max) return u64(1) << shift;
+    const double t = fma(double(v), scale, offset);  // 128 log2 of the weight
+    if (!(t >= lowest)) return 0;                    // rounds to none; -infinity, and what is infinitely far from the largest
+    const double m = t + 6755399441055744.0;         // 1.5 * 2^52: its low word is t rounded
+    const int n = __double2loint(m);
+    const double r = t - (m - 6755399441055744.0);   // |r| <= 1/2: 2^(r / 128) by its series, the fifth term is below 2^-49
+    constexpr double a1 = 0.0054152123481245725, a2 = a1 * a1 / 2, a3 = a1 * a1 * a1 / 6, a4 = a1 * a1 * a1 * a1 / 24;  // a1 = ln 2 / 128
+    const double q = r * fma(r, fma(r, fma(r, a4, a3), a2), a1), w = s->table[n & 127];
+    const double x = fma(w, q, w);                   // [1, 2) or just past it, times 2^(n >> 7)
+    const double y = __hiloint2double(__double2hiint(x) + (((n >> 7) + shift) << 20), __double2loint(x));
+    return static_cast<u64>(__double_as_longlong(y + 4503599627370496.0) - __double_as_longlong(4503599627370496.0));  // 2^52: rounded to a whole number
   }
-  __device__ __forceinline__ unsigned long long block_sum(unsigned long long v) {
+  __device__ __forceinline__ u64 block_sum(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
@@ -101,18 +123,18 @@ template <typename T> struct Row {
     return v;
   }
   // Running sum over the CTA's threads, v included, and the whole
-  __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long& whole) {
+  __device__ __forceinline__ u64 block_scan(u64 v, u64& whole) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+      const u64 u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += u;
     }
     __syncthreads();
     if (lane == 31) s->part[warp] = v;
     __syncthreads();
     whole = 0;
-    unsigned long long before = 0;
+    u64 before = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += s->part[w];
@@ -121,35 +143,26 @@ template <typename T> struct Row {
     return v + before;
   }
   // Every CTA's value in s->told[turn]: two turns, so that a CTA may tell the next while another still reads this one
-  __device__ __forceinline__ const unsigned long long* tell(unsigned long long v) {
+  __device__ __forceinline__ const u64* tell(u64 v) {
     turn ^= 1;
     cg::cluster_group cluster = cg::this_cluster();
-    if (threadIdx.x < ctas) cluster.map_shared_rank(s->told[turn], threadIdx.x)[rank] = v;
+    if (int(threadIdx.x) < ctas) cluster.map_shared_rank(s->told[turn], threadIdx.x)[rank_in] = v;
     cluster.sync();
     return s->told[turn];
   }
-  __device__ __forceinline__ unsigned long long cluster_sum(unsigned long long v, unsigned long long& before) {
-    const unsigned long long* all = tell(block_sum(v));
-    unsigned long long whole = 0;
-    before = 0;
-    for (int c = 0; c < ctas; ++c) {
-      if (c < rank) before += all[c];
-      whole += all[c];
-    }
-    return whole;
-  }
+  __device__ __forceinline__ u64 cluster_sum(u64 v, u64& before) { return totals(block_sum(v), before); }
   // The first index of the row at which the running sum of f reaches `need` (>= 1, at most the whole), which starts with `before` in this
   // CTA; all ones where that is not in this CTA's slice.
-  template <typename F> __device__ __forceinline__ uint32_t search(F&& f, unsigned long long before, unsigned long long need) {
+  template <typename F> __device__ __forceinline__ uint32_t search(F&& f, u64 before, u64 need) {
     if (threadIdx.x == 0) s->token = 0xffffffffu;
     if (before >= need) { __syncthreads(); return 0xffffffffu; }
     for (int b = begin; b < end; b += kThreads * 8) {  // uniform
       const int i = b + int(threadIdx.x) * 8;
-      unsigned long long mine = 0, whole;
+      u64 mine = 0, whole;
       each_of(i, [&](int j, float v) { mine += f(j, v); });
-      const unsigned long long to = block_scan(mine, whole) + before;
+      const u64 to = block_scan(mine, whole) + before;
       if (to >= need && to - mine < need) {
-        unsigned long long run = to - mine;
+        u64 run = to - mine;
         bool done = false;
         each_of(i, [&](int j, float v) {
           run += f(j, v);
@@ -163,23 +176,43 @@ template <typename T> struct Row {
     return s->token;
   }
 
-  // Narrows the kept tokens to the shortest prefix by size whose count (MASS: mass) reaches `need`.
-  template <bool MASS> __device__ void narrow(unsigned long long need, float lowest) {
+  // In the first CTA: the candidates of s->cand by size in s->sorted (up to `most` of them), `n` in all
+  __device__ __forceinline__ void rank(int n, int most) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const u64 mine = s->cand[i];
+      int before = 0;
+      for (int j = 0; j < n; ++j) before += s->cand[j] > mine;
+      if (before < most) s->sorted[before] = mine;
+    }
+    __syncthreads();
+  }
+  // An element to the first CTA's candidates
+  __device__ __forceinline__ void send(int i, uint32_t key) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t at = atomicAdd(cluster.map_shared_rank(&s->n_cand, 0), 1u);
+    if (at < kCandidates) cluster.map_shared_rank(s->cand, 0)[at] = (u64(key) << 32) | uint32_t(~i);
+  }
+
+  // Narrows the kept tokens to the shortest prefix by size whose count reaches `need`, or (MASS) whose mass reaches the fraction p of all of theirs.
+  template <bool MASS> __device__ void narrow(u64 need, double p, float least) {
     cg::cluster_group cluster = cg::this_cluster();
     uint32_t low = threshold > kNone ? threshold : kNone + 1, high = key_of(max);
-    unsigned long long above = 0, ties = 0;
-    const float scale = float(kBins) / (max - lowest);
-    bool linear = isfinite(scale) && scale > 0.f && max - lowest > 0.f && isfinite(max) && isfinite(lowest);
+    u64 above = 0, ties = 0;
+    const float per_bin = float(kBins) / (max - least);
+    bool linear = isfinite(per_bin) && per_bin > 0.f && max - least > 0.f && isfinite(max) && isfinite(least);
     bool first = true;
+    const int slice = kBins / ctas;  // bins that this CTA adds up over the cluster
     while (first || low < high) {
-      first = false;
       const uint32_t span = high - low;
-      const int shift = max_(0, 32 - __clz(span) - 11);
+      const int shift_of = max_(0, 32 - __clz(span) - 11);
       auto bin_of = [&](float v, uint32_t key) -> int {
         // both fall with the value, so a bin's tokens are next to each other by size
-        return linear ? min(kBins - 1, int(fminf((max - v) * scale, float(kBins)))) : int((high - key) >> shift);
+        return linear ? min(kBins - 1, int(fminf((max - v) * per_bin, float(kBins)))) : int((high - key) >> shift_of);
       };
-      for (int b = threadIdx.x; b < kBins; b += kThreads) { s->mass[b] = 0; s->count[b] = 0; }
+      for (int b = threadIdx.x; b < kBins; b += kThreads) {
+        s->count[b] = 0;
+        if (MASS) s->mass_low[b] = s->mass_high[b] = 0;
+      }
       __syncthreads();
       each([&](int i, float v) {
         const uint32_t key = key_of(v);
@@ -187,51 +220,108 @@ template <typename T> struct Row {
           const int b = bin_of(v, key);
           atomicAdd(&s->count[b], 1u);
           if (MASS) {
-            const unsigned long long w = mass_of(v);
-            if (w) atomicAdd(&s->mass[b], w);
+            const u64 w = mass_of(v);
+            if (w) {  // 64 bits by two atomics: whoever makes the low word overflow carries
+              const uint32_t lo = uint32_t(w), old = atomicAdd(&s->mass_low[b], lo), hi = uint32_t(w >> 32) + (old + lo < old ? 1u : 0u);
+              if (hi) atomicAdd(&s->mass_high[b], hi);
+            }
           }
         }
       });
+      if (threadIdx.x == 0) { s->n_cand = 0; s->low = 0xffffffffu; s->high = 0; s->bin = 0xffffffffu; }
       cluster.sync();
-      constexpr int kPer = kBins / kThreads;
-      unsigned long long metric[kPer], counts[kPer], mine = 0, whole;
+      // This CTA's bins, neighbouring ones by a thread
+      const int per = (slice + kThreads - 1) / kThreads, b0 = rank_of_slice(slice) + int(threadIdx.x) * per;
+      const bool has = int(threadIdx.x) * per < slice;
+      u64 metric[4], mine = 0;
+      uint32_t counts[4];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) metric[j] = counts[j] = 0;
-      for (int c = 0; c < ctas; ++c) {
-        const uint32_t* rc = cluster.map_shared_rank(s->count, c);
-        const unsigned long long* rm = cluster.map_shared_rank(s->mass, c);
+      for (int j = 0; j < 4; ++j) { metric[j] = 0; counts[j] = 0; }
+      if (has)
+        for (int c = 0; c < ctas; ++c) {
+          const uint32_t* rc = cluster.map_shared_rank(s->count, c);
+          const uint32_t* rl = cluster.map_shared_rank(s->mass_low, c);
+          const uint32_t* rh = cluster.map_shared_rank(s->mass_high, c);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          counts[j] += rc[threadIdx.x * kPer + j];
-          if (MASS) metric[j] += rm[threadIdx.x * kPer + j];
+          for (int j = 0; j < 4; ++j)
+            if (j < per) {
+              counts[j] += rc[b0 + j];
+              if (MASS) metric[j] += (u64(rh[b0 + j]) << 32) + rl[b0 + j];
+            }
         }
-      }
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
+      for (int j = 0; j < 4; ++j) {
         if (!MASS) metric[j] = counts[j];
         mine += metric[j];
       }
-      const unsigned long long to = block_scan(mine, whole) + above;
-      if (to >= need && to - mine < need) {
-        unsigned long long run = to - mine;
-        bool done = false;
+      u64 here, before;
+      const u64 to = block_scan(mine, here);
+      const u64 whole = totals(here, before);
+      if (MASS && first) {
+        const double want = ceil(p * double(whole));
+        need = want >= 1.0 ? static_cast<u64>(want) : 1ull;
+        if (need > whole) need = whole;
+      }
+      if (above + whole < need) return;  // all of them do not reach it: all stay (uniform over the cluster)
+      u64 run = above + before + to - mine;
+      if (run < need && run + mine >= need) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          if (!done && run + metric[j] >= need) {
-            s->bin = threadIdx.x * kPer + j;
-            s->bin_count = uint32_t(counts[j]);
+        for (int j = 0; j < 4; ++j) {
+          if (run < need && run + metric[j] >= need) {
+            s->bin = b0 + j;
+            s->bin_count = counts[j];
             s->above = run;
-            done = true;
           }
           run += metric[j];
         }
       }
-      if (threadIdx.x == 0) { s->low = 0xffffffffu; s->high = 0; }
       __syncthreads();
-      if (above + whole < need) return;  // all of them do not reach it: all stay (uniform over the cluster)
-      const int bin = int(s->bin);
-      ties = s->bin_count;
-      above = s->above;
+      // from the CTA that found it to all
+      const u64* where = tell((u64(s->bin) << 32) | s->bin_count);
+      int owner = 0;
+      for (int c = 0; c < ctas; ++c)
+        if (uint32_t(where[c] >> 32) != 0xffffffffu) owner = c;
+      const int bin = int(where[owner] >> 32);
+      ties = uint32_t(where[owner]);
+      above = tell(s->above)[owner];
+      first = false;
+      if (ties <= kCandidates && (linear || shift_of > 0)) {
+        // few: ranked by the first CTA
+        each([&](int i, float v) {
+          const uint32_t key = key_of(v);
+          if (key >= low && key <= high && kept(i, key) && bin_of(v, key) == bin) send(i, key);
+        });
+        cluster.sync();
+        if (rank_in == 0) {
+          const int n = int(ties);
+          this->rank(n, n);
+          u64 sum = 0;
+          const int per_thread = kCandidates / kThreads;
+          u64 w[per_thread];
+#pragma unroll
+          for (int j = 0; j < per_thread; ++j) {
+            const int i = int(threadIdx.x) * per_thread + j;
+            w[j] = i < n ? (MASS ? mass_of(of_key(uint32_t(s->sorted[i] >> 32))) : 1ull) : 0ull;
+            sum += w[j];
+          }
+          u64 all;
+          u64 at = above + block_scan(sum, all) - sum;
+#pragma unroll
+          for (int j = 0; j < per_thread; ++j) {
+            if (at < need && at + w[j] >= need) {
+              const u64 e = s->sorted[threadIdx.x * per_thread + j];
+              s->border_key = uint32_t(e >> 32);
+              s->border_index = ~uint32_t(e);
+            }
+            at += w[j];
+          }
+          __syncthreads();
+        }
+        const u64 border = tell((u64(s->border_key) << 32) | s->border_index)[0];
+        threshold = uint32_t(border >> 32);
+        last = int(uint32_t(border));
+        return;
+      }
       if (linear) {  // the keys of that bin
         uint32_t lo = 0xffffffffu, hi = 0;
         each([&](int i, float v) {
@@ -241,30 +331,29 @@ template <typename T> struct Row {
         atomicMin(&s->low, lo);
         atomicMax(&s->high, hi);
         __syncthreads();
-        const unsigned long long* all = tell((static_cast<unsigned long long>(s->low) << 32) | s->high);
+        const u64* all = tell((u64(s->low) << 32) | s->high);
         low = 0xffffffffu;
         high = 0;
         for (int c = 0; c < ctas; ++c) { low = min(low, uint32_t(all[c] >> 32)); high = max_(high, uint32_t(all[c])); }
         linear = false;
       } else {
-        const uint32_t top = high - (uint32_t(bin) << shift), width = 1u << shift;
+        const uint32_t top = high - (uint32_t(bin) << shift_of), width = 1u << shift_of;
         low = top - low >= width ? top - width + 1 : low;
         high = top;
-        cluster.sync();  // the bins are cleared next: all have read them
       }
     }
     // `ties` tokens have the key `low`; so many of them are needed
-    const unsigned long long w = MASS ? mass_of(of_key(low)) : 1ull;
-    const unsigned long long n = w ? (need - above + w - 1) / w : 1ull;
+    const u64 w = MASS ? mass_of(of_key(low)) : 1ull;
+    const u64 n = w ? (need - above + w - 1) / w : 1ull;
     int cut = INT_MAX;
     if (n < ties) {
       const int old_last = low == threshold ? last : INT_MAX;
-      auto tie = [&](int i, float v) -> unsigned long long { return key_of(v) == low && i <= old_last ? 1ull : 0ull; };
-      unsigned long long mine = 0, before;
+      auto tie = [&](int i, float v) -> u64 { return key_of(v) == low && i <= old_last ? 1ull : 0ull; };
+      u64 mine = 0, before;
       each([&](int i, float v) { mine += tie(i, v); });
       cluster_sum(mine, before);
       const uint32_t at = search(tie, before, n);
-      const unsigned long long* all = tell(at);
+      const u64* all = tell(at);
       uint32_t where = 0xffffffffu;
       for (int c = 0; c < ctas; ++c) where = min(where, uint32_t(all[c]));
       cut = int(where);
@@ -274,53 +363,72 @@ template <typename T> struct Row {
     threshold = low;
     last = cut;
   }
+  __device__ __forceinline__ int rank_of_slice(int slice) const { return rank_in * slice; }
+  // The sum over the cluster of a value that is the same in all threads of a CTA, and what the CTAs before this one have of it
+  __device__ __forceinline__ u64 totals(u64 v, u64& before) {
+    const u64* all = tell(v);
+    u64 whole = 0;
+    before = 0;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank_in) before += all[c];
+      whole += all[c];
+    }
+    return whole;
+  }
   static __device__ __forceinline__ int max_(int a, int b) { return a > b ? a : b; }
   static __device__ __forceinline__ uint32_t max_(uint32_t a, uint32_t b) { return a > b ? a : b; }
 };
 
 // How much mass the running sum has to reach: the first sum above u * whole is the first that is >= this
-__device__ __forceinline__ unsigned long long to_reach(double u, unsigned long long whole) {
+__device__ __forceinline__ u64 to_reach(double u, u64 whole) {
   const double t = floor(u * double(whole));
-  const unsigned long long n = t > 0 ? static_cast<unsigned long long>(t) + 1 : 1ull;
+  const u64 n = t > 0 ? static_cast<u64>(t) + 1 : 1ull;
   return n < whole ? n : whole;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs p) {
-  __shared__ Shared s;
+  extern __shared__ __align__(16) uint8_t dynamic[];
+  Shared& s = *reinterpret_cast<Shared*>(dynamic);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank()), row = int(blockIdx.x) / ctas;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
   Row<T> r;
   r.x = reinterpret_cast<const T*>(p.logits) + int64_t(row) * p.row_stride;
   r.begin = int(min(int64_t(p.vocab), int64_t(rank) * p.per_cta));
   r.end = int(min(int64_t(p.vocab), int64_t(r.begin) + p.per_cta));
-  r.rank = rank; r.ctas = ctas; r.turn = 0; r.vec = p.vec != 0; r.s = &s;
+  r.rank_in = rank; r.ctas = ctas; r.turn = 0; r.vec = p.vec != 0; r.s = &s;
   const float t = p.temperature ? p.temperature[row] : 1.f;
   const bool greedy = !p.uniforms || !(t > 0.f);
+  const int k = p.top_k ? p.top_k[row] : 0;
+  if (threadIdx.x < 128) s.table[threadIdx.x] = exp2(double(threadIdx.x) * (1.0 / 128));
+  if (threadIdx.x == 0) s.n_cand = 0;
 
-  // the largest logit
-  unsigned long long best = 0;
+  // the largest logit, of 256 groups of them; the smallest finite one
+  u64 best = 0;
   float least = INFINITY;
   r.each([&](int i, float v) {
-    const unsigned long long e = (static_cast<unsigned long long>(key_of(v)) << 32) | uint32_t(~i);
+    const u64 e = (u64(key_of(v)) << 32) | uint32_t(~i);
     if (i < r.end) {
       best = best > e ? best : e;
       if (v > -INFINITY) least = fminf(least, v);
     }
   });
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long e = __shfl_xor_sync(0xffffffffu, best, o);
+  const int width = 2 * ctas;  // lanes of a group: 256 / ctas groups in a CTA
+  for (int o = width >> 1; o > 0; o >>= 1) {
+    const u64 e = __shfl_xor_sync(0xffffffffu, best, o);
     best = best > e ? best : e;
   }
-  if (lane < ctas) cluster.map_shared_rank(s.warp_max, lane)[rank * kWarps + warp] = best;
+  {
+    const int groups = kGroups / ctas, group = int(threadIdx.x) / width;
+    for (int c = lane & (width - 1); c < ctas; c += width) cluster.map_shared_rank(s.group_max, c)[rank * groups + group] = best;
+  }
   cluster.sync();
-  unsigned long long top = 0;
-  for (int w = lane; w < ctas * kWarps; w += 32) top = top > s.warp_max[w] ? top : s.warp_max[w];
+  u64 top = 0;
+  for (int w = lane; w < kGroups; w += 32) top = top > s.group_max[w] ? top : s.group_max[w];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long e = __shfl_xor_sync(0xffffffffu, top, o);
+    const u64 e = __shfl_xor_sync(0xffffffffu, top, o);
     top = top > e ? top : e;
   }
   if (uint32_t(top >> 32) <= kNone || greedy) {  // the same in all CTAs of the row
@@ -328,8 +436,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs p) {
     return;
   }
   r.max = of_key(uint32_t(top >> 32));
-  r.inv_t = 1.0 / double(t);
-  r.one = ldexp(1.0, p.shift);
+  r.shift = p.shift;
+  r.scale = 128 * 1.4426950408889634 / double(t);
+  r.offset = -double(r.max) * r.scale;
+  r.lowest = -128.0 * (p.shift + 1);
   r.threshold = kNone;
   r.last = -1;
   r.min_key = 0;
@@ -341,40 +451,76 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs p) {
   }
   float u = p.uniforms[row];
   u = u > 0.f ? fminf(u, 1.f) : 0.f;
-  const int k = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
 
-  if (k > 0 && k < p.vocab) {
-    float lowest = 0.f;
+  if (k > 0 && k <= kMaxQuick && k < p.vocab) {
+    // The k-th largest of the groups' maxima: at least k logits are not below it
+    if (threadIdx.x == 0) s.low = kNone + 1;
+    __syncthreads();
     {
-      // the smallest finite logit of the row
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-      if (threadIdx.x == 0) s.low = 0xffffffffu;
-      __syncthreads();
-      if (lane == 0) atomicMin(&s.low, key_of(least));
-      __syncthreads();
-      const unsigned long long* all = r.tell(s.low);
-      uint32_t lo = 0xffffffffu;
-      for (int c = 0; c < ctas; ++c) lo = min(lo, uint32_t(all[c]));
-      lowest = of_key(lo);
+      const int g = int(threadIdx.x) >> 1, half = threadIdx.x & 1;
+      const u64 mine = s.group_max[g];
+      int before = 0;
+      for (int j = half * (kGroups / 2); j < (half + 1) * (kGroups / 2); ++j) before += s.group_max[j] > mine;
+      before += __shfl_xor_sync(0xffffffffu, before, 1);
+      if (half == 0 && before == k - 1 && uint32_t(mine >> 32) > kNone) s.low = uint32_t(mine >> 32);
     }
-    r.template narrow<false>(static_cast<unsigned long long>(k), lowest);
+    __syncthreads();
+    const uint32_t from = s.low;
+    r.each([&](int i, float v) {
+      const uint32_t key = key_of(v);
+      if (key >= from) r.send(i, key);
+    });
+    cluster.sync();
+    const int n = int(*cluster.map_shared_rank(&s.n_cand, 0));
+    if (n <= kCandidates) {
+      if (rank == 0) {
+        const int kept = min(k, n), i = threadIdx.x;
+        r.rank(n, kept);
+        const u64 e = i < kept ? s.sorted[i] : 0;
+        u64 w = i < kept ? r.mass_of(of_key(uint32_t(e >> 32))) : 0, whole;
+        if (top_p < 1.f) {
+          const u64 to = r.block_scan(w, whole);
+          const double want = ceil(double(fmaxf(top_p, 0.f)) * double(whole));
+          if (to - w >= (want >= 1.0 ? static_cast<u64>(want) : 1ull)) w = 0;
+        }
+        if (uint32_t(e >> 32) < r.min_key) w = 0;
+        s.weight[i] = w;
+        whole = r.block_sum(w);
+        const u64 need = to_reach(double(u), whole);
+        if (w) {  // the running mass in the order of the vocabulary
+          u64 before = 0;
+          for (int j = 0; j < kept; ++j) before += uint32_t(s.sorted[j]) > uint32_t(e) ? s.weight[j] : 0;  // ~index
+          if (before < need && before + w >= need) p.out[row] = int(~uint32_t(e));
+        }
+      }
+      cluster.sync();  // the count has been read by all
+      return;
+    }
+    cluster.sync();
   }
-  if (top_p < 1.f) {
-    unsigned long long mine = 0, before;
-    r.each([&](int i, float v) { if (r.kept(i, key_of(v))) mine += r.mass_of(v); });
-    const unsigned long long whole = r.cluster_sum(mine, before);
-    const double want = ceil(double(fmaxf(top_p, 0.f)) * double(whole));
-    r.template narrow<true>(want >= 1.0 ? static_cast<unsigned long long>(want) : 1ull, r.max - 31.f * t);
+  if (k > 0 && k < p.vocab) {
+    // the smallest finite logit of the row
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+    __syncthreads();
+    if (threadIdx.x == 0) s.low = 0xffffffffu;
+    __syncthreads();
+    if (lane == 0) atomicMin(&s.low, key_of(least));
+    __syncthreads();
+    const u64* all = r.tell(s.low);
+    uint32_t lo = 0xffffffffu;
+    for (int c = 0; c < ctas; ++c) lo = min(lo, uint32_t(all[c]));
+    r.template narrow<false>(u64(k), 0.0, of_key(lo));
   }
-  auto weight = [&](int i, float v) -> unsigned long long {
+  if (top_p < 1.f) r.template narrow<true>(0, double(fmaxf(top_p, 0.f)), r.max - 31.f * t);
+  auto weight = [&](int i, float v) -> u64 {
     const uint32_t key = key_of(v);
     return key >= r.min_key && r.kept(i, key) ? r.mass_of(v) : 0ull;
   };
-  unsigned long long mine = 0, before;
+  u64 mine = 0, before;
   r.each([&](int i, float v) { mine += weight(i, v); });
-  const unsigned long long whole = r.cluster_sum(mine, before);
+  const u64 whole = r.cluster_sum(mine, before);
   const uint32_t token = r.search(weight, before, to_reach(double(u), whole));
   if (threadIdx.x == 0 && token != 0xffffffffu) p.out[row] = int(token);
 }
@@ -401,14 +547,19 @@ int32_t tl_sample(tl_ctx* ctx, const void* logits, int32_t dtype, int64_t rows, 
   p.vocab = int32_t(vocab);
   p.shift = 44;
   while (p.shift > 38 && (vocab >> (62 - p.shift)) != 0) --p.shift;  // the whole mass stays below 2^63
+  // CTAs of a row: as many as keep all rows in one wave of two CTAs an SM, each with a vector a thread
   int ctas = 1;
-  while (ctas < 8 && vocab > int64_t(ctas) * kThreads * 8) ctas *= 2;
+  while (ctas < kMaxCluster && vocab > int64_t(ctas) * kThreads * 8 && rows * ctas * 2 <= 2 * int64_t(ctx->sm_count)) ctas *= 2;
   p.per_cta = int32_t(((vocab + ctas - 1) / ctas + 7) / 8 * 8);
   const size_t esz = tl_dtype_size(dtype);
   p.vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && (rows == 1 || (row_stride * int64_t(esz)) % 16 == 0);
+  const auto kernel = dtype == TL_F32 ? sample_kernel<float> : dtype == TL_F16 ? sample_kernel<__half> : sample_kernel<__nv_bfloat16>;
+  TL_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Shared))));
+  if (ctas > 8) TL_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(rows * ctas));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -416,8 +567,7 @@ int32_t tl_sample(tl_ctx* ctx, const void* logits, int32_t dtype, int64_t rows, 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  TL_CUDA(ctx, dtype == TL_F32 ? cudaLaunchKernelEx(&cfg, sample_kernel<float>, p)
-                               : dtype == TL_F16 ? cudaLaunchKernelEx(&cfg, sample_kernel<__half>, p) : cudaLaunchKernelEx(&cfg, sample_kernel<__nv_bfloat16>, p));
+  TL_CUDA(ctx, cudaLaunchKernelEx(&cfg, kernel, p));
   ctx->counters[TL_COUNTER_KERNEL_LAUNCHES]++;
   tl_wrote(ctx, out_tokens, rows * int64_t(sizeof(int32_t)));
   return TL_OK;
