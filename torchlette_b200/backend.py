@@ -175,19 +175,19 @@ class PagedCache:
         self.nPages, self.kvHeads, self.pageSize, self.headDim = kPages.shape
         self.nSeqs, self.maxPages = pageTable.shape
         self._shape = (self.nPages, self.pageSize, self.kvHeads, self.headDim, B.DTYPE_ID[self.dtype], self.nSeqs, self.maxPages)
-        self._bytes = self._at = None
+        self._bytes = self._k = self._v = self._table = None
 
     def descriptor(self) -> bytes:
         """The cache as the bytes of a tl_paged_cache."""
-        at = (self.kPages.buffer, self.vPages.buffer, self.pageTable.buffer)
-        if at != self._at:  # the first call, or a tensor was given another buffer
-            self._bytes, self._at = bytes(B.PagedCache(*at, *self._shape)), at
+        k, v, table = self.kPages.buffer, self.vPages.buffer, self.pageTable.buffer
+        if k != self._k or v != self._v or table != self._table:  # the first call, or a tensor was given another buffer
+            self._bytes = bytes(B.PagedCache(k, v, table, *self._shape))
+            self._k, self._v, self._table = k, v, table
         return self._bytes
 
 
-def _needs(ok: bool, message: str):
-    if not ok:
-        raise TlError(B.TL_ERR_INVALID_ARG, message)
+def _refuse(message: str):
+    raise TlError(B.TL_ERR_INVALID_ARG, message)
 
 
 class CudaOps:
@@ -348,11 +348,12 @@ class CudaOps:
         self._b._calls.tl_copy2d(self._b._handle, cache.buffer + position * d * esz, cap * d * esz, new.buffer, d * esz, d * esz, b * kvh)
 
     # -- a decode step over a paged cache (sequences of their own lengths) ----------
-    def _tokens(self, who: str, cache: PagedCache, positions: CudaTensor, tokenSeq: Optional[CudaTensor]) -> int:
-        _needs(positions.dtype == "i32" and len(positions.shape) == 1, f"{who}: positions are i32 [tokens]")
-        tokens = positions.shape[0]
-        _needs(tokenSeq is None or (tokenSeq.dtype == "i32" and tokenSeq.shape == [tokens]), f"{who}: tokenSeq is i32 [tokens]")
-        return tokens
+    def _tokens(self, who: str, positions: CudaTensor, tokenSeq: Optional[CudaTensor]) -> int:
+        if positions.dtype != "i32" or len(positions.shape) != 1:
+            _refuse(f"{who}: positions are i32 [tokens]")
+        if tokenSeq is not None and (tokenSeq.dtype != "i32" or tokenSeq.shape != positions.shape):
+            _refuse(f"{who}: tokenSeq is i32 [tokens]")
+        return positions.shape[0]
 
     def pagedAppend(self, cache: PagedCache, positions: CudaTensor, q: Optional[CudaTensor], k: Optional[CudaTensor], v: Optional[CudaTensor],
                     cos: Optional[CudaTensor] = None, sin: Optional[CudaTensor] = None, *, qNorm: Optional[CudaTensor] = None,
@@ -363,48 +364,54 @@ class CudaOps:
         [T, H * D], k and v [T, kvH, D] or [T, kvH * D]; with ``headsFirst`` all of them, the result too, are [heads, T, D] (the order of
         fusedRoPE and attention).  k = v = None: q holds the rows of one product, [T, (H + 2 kvH) * D].  q = None: k and v alone.
         positions i32 [T], negative for tokens that are not there; tokenSeq i32 [T] their sequences (None: token t is of sequence t)."""
-        tokens, d, g = self._tokens("pagedAppend", cache, positions, tokenSeq), cache.headDim, cache.kvHeads
-        dtype, esz = cache.dtype, _ITEMSIZE[cache.dtype]
+        tokens, d, g, dtype = self._tokens("pagedAppend", positions, tokenSeq), cache.headDim, cache.kvHeads, cache.dtype
         for t in (q, k, v, out):
-            _needs(t is None or (t.dtype == dtype and not t.transposed), "pagedAppend: q, k, v and out have the cache's dtype")
+            if t is not None and (t.dtype != dtype or t.transposed):
+                _refuse("pagedAppend: q, k, v and out have the cache's dtype")
         if k is None and v is None:
-            _needs(q is not None and not headsFirst and len(q.shape) == 2 and q.shape[0] == tokens and q.shape[1] % d == 0 and q.shape[1] > 2 * g * d,
-                   "pagedAppend: q alone is [tokens, (H + 2 kvH) * D]")
-            width = q.shape[1]
-            heads = width // d - 2 * g
-            q_at, k_at, v_at = q.buffer, q.buffer + heads * d * esz, q.buffer + (heads + g) * d * esz
-            strides = kv_strides = (width, d)
+            if q is None or headsFirst or len(q.shape) != 2 or q.shape[0] != tokens or q.shape[1] % d or q.shape[1] <= 2 * g * d:
+                _refuse("pagedAppend: q alone is [tokens, (H + 2 kvH) * D]")
+            ts = k_ts = q.shape[1]
+            hs = k_hs = d
+            heads, esz = ts // d - 2 * g, _ITEMSIZE[dtype]
+            q_at = q.buffer
+            k_at = q_at + heads * d * esz
+            v_at = k_at + g * d * esz
         else:
-            _needs(k is not None and v is not None, "pagedAppend: k and v come together")
+            if k is None or v is None:
+                _refuse("pagedAppend: k and v come together")
             shapes = ([g, tokens, d],) if headsFirst else ([tokens, g, d], [tokens, g * d])
-            _needs(list(k.shape) in shapes and list(v.shape) in shapes, f"pagedAppend: k and v are {shapes[0]}")
-            kv_strides = (d, tokens * d) if headsFirst else (g * d, d)
-            k_at, v_at, q_at, heads, strides = k.buffer, v.buffer, None, 0, (0, 0)
+            if k.shape not in shapes or v.shape not in shapes:
+                _refuse(f"pagedAppend: k and v are {shapes[0]}")
+            k_ts, k_hs = (d, tokens * d) if headsFirst else (g * d, d)
+            k_at, v_at, q_at, heads, ts, hs = k.buffer, v.buffer, None, 0, 0, 0
             if q is not None:
-                heads = q.shape[0] if headsFirst else int(math.prod(q.shape[1:])) // d
-                _needs(heads > 0 and list(q.shape) in (([heads, tokens, d],) if headsFirst else ([tokens, heads, d], [tokens, heads * d])),
-                       "pagedAppend: q is [tokens, H, D]")
-                q_at, strides = q.buffer, (d, tokens * d) if headsFirst else (heads * d, d)
-        for t in (qNorm, kNorm):
-            _needs(t is None or list(t.shape) == [d], "pagedAppend: qNorm and kNorm are [D]")
-        _needs(qNorm is None or kNorm is None or qNorm.dtype == kNorm.dtype, "pagedAppend: qNorm and kNorm have one dtype")
+                shape = q.shape
+                heads = shape[0] if headsFirst else shape[1] if len(shape) == 3 else shape[1] // d if len(shape) == 2 else 0
+                if heads < 1 or shape not in (([heads, tokens, d],) if headsFirst else ([tokens, heads, d], [tokens, heads * d])):
+                    _refuse("pagedAppend: q is [tokens, H, D]")
+                q_at = q.buffer
+                ts, hs = (d, tokens * d) if headsFirst else (heads * d, d)
         norm = qNorm if qNorm is not None else kNorm
-        _needs((cos is None) == (sin is None), "pagedAppend: cos and sin come together")
-        if cos is not None:
-            _needs(cos.dtype == sin.dtype == "f32" and len(cos.shape) == 2 and cos.shape == sin.shape and 2 * cos.shape[1] == d,
-                   "pagedAppend: cos and sin are f32 [rows, D/2]")
+        if norm is not None and (norm.shape != [d] or (kNorm is not None and (kNorm.shape != [d] or kNorm.dtype != norm.dtype)) or norm.dtype not in B.DTYPE_ID):
+            _refuse("pagedAppend: qNorm and kNorm are [D] of one dtype")
+        if (cos is None) != (sin is None):
+            _refuse("pagedAppend: cos and sin come together")
+        if cos is not None and (cos.dtype != "f32" or sin.dtype != "f32" or len(cos.shape) != 2 or cos.shape != sin.shape or 2 * cos.shape[1] != d):
+            _refuse("pagedAppend: cos and sin are f32 [rows, D/2]")
         if q_at is None:
-            _needs(out is None, "pagedAppend: out is the new q's")
+            if out is not None:
+                _refuse("pagedAppend: out is the new q's")
         else:
             shape = [heads, tokens, d] if headsFirst else [tokens, heads, d]
             if out is None:
                 out = self.empty(shape, dtype)
-            else:
-                _needs(list(out.shape) in (shape, [tokens, heads * d] if not headsFirst else shape), "pagedAppend: out is q's shape")
-        out_strides = (d, tokens * d) if headsFirst else (heads * d, d)
+            elif out.shape != shape and (headsFirst or out.shape != [tokens, heads * d]):
+                _refuse("pagedAppend: out is q's shape")
+        o_ts, o_hs = (d, tokens * d) if headsFirst else (heads * d, d)
         self._b._calls.tl_paged_append(
-            self._b._handle, cache.descriptor(), positions.buffer, tokenSeq.buffer if tokenSeq is not None else None, tokens, q_at, *strides, heads,
-            out.buffer if out is not None else None, *out_strides, k_at, *kv_strides, v_at, *kv_strides,
+            self._b._handle, cache.descriptor(), positions.buffer, tokenSeq.buffer if tokenSeq is not None else None, tokens, q_at, ts, hs, heads,
+            out.buffer if out is not None else None, o_ts, o_hs, k_at, k_ts, k_hs, v_at, k_ts, k_hs,
             qNorm.buffer if qNorm is not None else None, kNorm.buffer if kNorm is not None else None,
             B.DTYPE_ID[norm.dtype] if norm is not None else 0, float(eps), cos.buffer if cos is not None else None,
             sin.buffer if sin is not None else None, cos.shape[0] if cos is not None else 0)
@@ -415,16 +422,16 @@ class CudaOps:
         """softmax(cap(q k^T * scale) + slope * (j - p)) v of each token over its own sequence's positions j <= p (with ``window``: the last
         ``window`` of them), p = positions[t] and among the appended ones.  q [T, H, D] or [T, H * D]; returns [T, H * D], the layout o_proj
         reads, zeros for tokens that are not there (a negative position).  softcap 0: no cap; slopes f32 [H]; tokenSeq as in pagedAppend."""
-        tokens, d = self._tokens("pagedAttention", cache, positions, tokenSeq), cache.headDim
-        heads = int(math.prod(q.shape[1:])) // d
-        _needs(heads > 0 and list(q.shape) in ([tokens, heads, d], [tokens, heads * d]) and q.dtype == cache.dtype and not q.transposed,
-               "pagedAttention: q is [tokens, H, D] of the cache's dtype")
-        _needs(slopes is None or (slopes.dtype == "f32" and list(slopes.shape) == [heads]), "pagedAttention: slopes are f32 [H]")
+        tokens, d, shape = self._tokens("pagedAttention", positions, tokenSeq), cache.headDim, q.shape
+        heads = shape[1] if len(shape) == 3 else shape[1] // d if len(shape) == 2 else 0
+        if heads < 1 or (shape != [tokens, heads, d] and shape != [tokens, heads * d]) or q.dtype != cache.dtype or q.transposed:
+            _refuse("pagedAttention: q is [tokens, H, D] of the cache's dtype")
+        if slopes is not None and (slopes.dtype != "f32" or slopes.shape != [heads]):
+            _refuse("pagedAttention: slopes are f32 [H]")
         if out is None:
             out = self.empty([tokens, heads * d], cache.dtype)
-        else:
-            _needs(out.dtype == cache.dtype and not out.transposed and list(out.shape) in ([tokens, heads * d], [tokens, heads, d]),
-                   "pagedAttention: out is [tokens, H * D] of the cache's dtype")
+        elif out.dtype != cache.dtype or out.transposed or (out.shape != [tokens, heads * d] and out.shape != [tokens, heads, d]):
+            _refuse("pagedAttention: out is [tokens, H * D] of the cache's dtype")
         self._b._calls.tl_paged_attention(self._b._handle, cache.descriptor(), positions.buffer, tokenSeq.buffer if tokenSeq is not None else None,
                                           tokens, q.buffer, heads * d, d, heads, out.buffer, float(scale), float(softcap), int(window),
                                           slopes.buffer if slopes is not None else None)
@@ -438,16 +445,22 @@ class CudaOps:
         the first index whose running mass exceeds uniforms times the whole.  Each parameter is f32 (topK: i32) [rows] or None (off).
         temperature <= 0, or no uniforms: the largest logit, the lowest index of equal ones.  -1 for a row that is all -infinity or NaN.
         Returns i32 [rows]."""
-        _needs(len(logits.shape) >= 1 and not logits.transposed, "sample: logits are [rows, vocab]")
+        if len(logits.shape) < 1 or logits.transposed or logits.dtype not in B.DTYPE_ID:
+            _refuse("sample: logits are [rows, vocab] of f32, f16 or bf16")
         rows, vocab = int(math.prod(logits.shape[:-1])), logits.shape[-1]
-        for t, name, dtype in ((uniforms, "uniforms", "f32"), (temperature, "temperature", "f32"), (topK, "topK", "i32"), (topP, "topP", "f32"),
-                               (minP, "minP", "f32"), (out, "out", "i32")):
-            _needs(t is None or (t.dtype == dtype and list(t.shape) == [rows]), f"sample: {name} is {dtype} [rows]")
-        _needs(logits.dtype in B.DTYPE_ID, f"sample: logits of dtype {logits.dtype}")
+        row = [rows]
+        for t in (uniforms, temperature, topP, minP):
+            if t is not None and (t.dtype != "f32" or t.shape != row):
+                _refuse("sample: uniforms, temperature, topP and minP are f32 [rows]")
+        for t in (topK, out):
+            if t is not None and (t.dtype != "i32" or t.shape != row):
+                _refuse("sample: topK and out are i32 [rows]")
         if out is None:
-            out = self.empty([rows], "i32")
-        at = [t.buffer if t is not None else None for t in (temperature, topK, topP, minP, uniforms)]
-        self._b._calls.tl_sample(self._b._handle, logits.buffer, B.DTYPE_ID[logits.dtype], rows, vocab, vocab, *at, out.buffer)
+            out = self.empty(row, "i32")
+        self._b._calls.tl_sample(self._b._handle, logits.buffer, B.DTYPE_ID[logits.dtype], rows, vocab, vocab,
+                                 temperature.buffer if temperature is not None else None, topK.buffer if topK is not None else None,
+                                 topP.buffer if topP is not None else None, minP.buffer if minP is not None else None,
+                                 uniforms.buffer if uniforms is not None else None, out.buffer)
         return out
 
     def matmul(self, a: CudaTensor, b: CudaTensor, options: Optional[dict] = None) -> CudaTensor:

@@ -7,9 +7,9 @@
 // f32 arithmetic, one rounding at the store; v is copied bit for bit.
 //
 // Bound: HBM for prompts (every element is read and written once), launch and the chain position -> page -> store for a step's few tokens.  A head
-// is a group of lanes, 8 dimensions each, which exchange halves by shuffles; a thread keeps its dimensions' rotation and norm weights in registers
-// and takes several heads of its token, whose loads are on their way together.
+// is a group of lanes; a thread keeps its dimensions' rotation in registers and takes several heads of its token, whose loads are on their way together.
 #include <algorithm>
+#include <type_traits>
 
 #include "tl_vec.cuh"
 
@@ -97,95 +97,117 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs p) {
   }
 }
 
-// Eight elements as they are stored
-template <typename T> struct Eight {
-  uint4 u[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
+// Four elements as they are stored
+template <typename T> struct Four {
+  using Bits = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
+  Bits u;
+  __device__ __forceinline__ void load(const T* p) { u = __ldcs(reinterpret_cast<const Bits*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Bits*>(p) = u; }
+  __device__ __forceinline__ void values(float (&v)[4]) const {
 #pragma unroll
-    for (int i = 0; i < int(sizeof(T)) / 2; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    for (int e = 0; e < 4; ++e) v[e] = DT<T>::to_f32(reinterpret_cast<const T*>(&u)[e]);
   }
-  __device__ __forceinline__ void store(T* p) const {
+  __device__ __forceinline__ void take(const float (&v)[4]) {
+    T e[4];
 #pragma unroll
-    for (int i = 0; i < int(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
-  }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = DT<T>::to_f32(reinterpret_cast<const T*>(u)[e]);
+    for (int i = 0; i < 4; ++i) e[i] = DT<T>::from_f32(v[i]);
+    u = *reinterpret_cast<const Bits*>(e);
   }
 };
-// Rows of whole 16-byte vectors: a group of LANES lanes (a power of two that holds head_dim / 8) a head, HEADS heads a thread, a CTA for a token's next
-// kThreads / LANES * HEADS heads.  The rows are held as stored until their turn, so that five CTAs an SM have loads on their way: 8001 tokens x 48 heads x
-// 128 bf16 (197 MB) took 115 us with 99 registers a thread and two CTAs.
+__device__ __forceinline__ void load4_any(const void* p, int dtype, int i, float (&v)[4]) {
+  if (dtype == TL_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else if (dtype == TL_F16) {
+    Four<__half> f;
+    f.u = *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p) + i);
+    f.values(v);
+  } else {
+    Four<__nv_bfloat16> f;
+    f.u = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+    f.values(v);
+  }
+}
+// A group of LANES lanes (a power of two that holds head_dim / 8) a head, HEADS heads a thread, a CTA for a token's next kThreads / LANES * HEADS heads.  A
+// lane has four dimensions of the first half and the same four of the second, which the rotation mixes: no lane needs another's.  The rows are held as
+// stored until their turn, so that several CTAs an SM have loads on their way.  (Eight neighbouring dimensions a lane and shuffles: 52 us for
+// 8001 tokens x 48 heads x 128 bf16, 197 MB, by the instructions that it issued.)
 constexpr int kThreads = 256;
 template <typename T, int LANES, int HEADS>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) append_vec_kernel(const __grid_constant__ AppendArgs p) {
   tl_pdl_wait();
   const int64_t t = blockIdx.x;
-  const int l = threadIdx.x % LANES, vectors = p.head_dim >> 3, half = vectors >> 1, d = 8 * l;
+  const int half = p.head_dim >> 1, d = 4 * int(threadIdx.x % LANES);
   const int n_q = p.q ? p.n_heads : 0, n_qk = n_q + p.n_kv_heads, rows = n_qk + p.n_kv_heads;
   constexpr int kStep = kThreads / LANES;
   const int first = int(blockIdx.y) * (kStep * HEADS) + int(threadIdx.x) / LANES;
-  const bool lane_in = l < vectors;
+  const bool lane_in = d < half;
 
   int pos = p.positions[t];  // asked for before the rows: the page and the rotation wait for it
-  Eight<T> x[HEADS];
+  Four<T> x[HEADS][2];
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
     const int r = first + i * kStep;
-    if (lane_in && r < rows)
-      x[i].load(r < n_q ? reinterpret_cast<const T*>(p.q) + t * p.qt + r * p.qh + d
-                        : r < n_qk ? reinterpret_cast<const T*>(p.k) + t * p.kt + (r - n_q) * p.kh + d
-                                   : reinterpret_cast<const T*>(p.v) + t * p.vt + (r - n_qk) * p.vh + d);
+    if (lane_in && r < rows) {
+      const T* from = (r < n_q ? reinterpret_cast<const T*>(p.q) + t * p.qt + r * p.qh
+                               : r < n_qk ? reinterpret_cast<const T*>(p.k) + t * p.kt + (r - n_q) * p.kh
+                                          : reinterpret_cast<const T*>(p.v) + t * p.vt + (r - n_qk) * p.vh) + d;
+      x[i][0].load(from);
+      x[i][1].load(from + half);
+    }
   }
   int64_t at;
   if (!place(p, t, pos, at)) return;  // the same in all threads
-  float c[8], s[8];
+  float c[4], s[4];
   if (lane_in && p.cos_t) {
-    const int64_t row = int64_t(pos) * (p.head_dim >> 1) + 8 * (l < half ? l : l - half);
-    load8(p.cos_t + row, c);
-    load8(p.sin_t + row, s);
-    if (l < half)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = -s[e];
+    load4_any(p.cos_t + int64_t(pos) * half, TL_F32, d, c);
+    load4_any(p.sin_t + int64_t(pos) * half, TL_F32, d, s);
   }
-  const int partner = l < half ? l + half : l < vectors ? l - half : l;
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
     const int r = first + i * kStep;
     const bool here = lane_in && r < rows, is_q = r < n_q, is_v = r >= n_qk;
     const void* weight = is_q ? p.q_weight : p.k_weight;
-    float y[8];
-    if (here) x[i].values(y);
+    float a[4], b[4], inv = 1.f;
+    if (here && !is_v) {
+      x[i][0].values(a);
+      x[i][1].values(b);
+    }
     if (p.q_weight || p.k_weight) {
       float ss = 0.f;
-      if (here)
+      if (here && !is_v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+        for (int e = 0; e < 4; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, LANES);
-      if (here && !is_v && weight) {
-        const float inv = rsqrtf(ss / float(p.head_dim) + p.eps);
-        float w[8];
-        load8_any(weight, p.w_dtype, d, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * w[e];
-      }
-    }
-    if (p.cos_t) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_sync(0xffffffffu, y[e], partner, LANES);
-        y[e] = fmaf(other, s[e], y[e] * c[e]);
-      }
+      inv = rsqrtf(ss / float(p.head_dim) + p.eps);
     }
     if (!here) continue;
-    if (is_q) {
-      store8(reinterpret_cast<T*>(p.q_out) + t * p.ot + r * p.oh + d, y);
-    } else if (at >= 0) {
-      T* to = reinterpret_cast<T*>(is_v ? p.v_pages : p.k_pages) + at + int64_t(is_v ? r - n_qk : r - n_q) * p.page_size * p.head_dim + d;
-      if (is_v) x[i].store(to);
-      else store8(to, y);
+    if (!is_v) {
+      if (weight) {
+        float w[4];
+        load4_any(weight, p.w_dtype, d, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = a[e] * inv * w[e];
+        load4_any(weight, p.w_dtype, d + half, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = b[e] * inv * w[e];
+      }
+      if (p.cos_t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = a[e] * c[e] - b[e] * s[e];
+          b[e] = b[e] * c[e] + a[e] * s[e];
+          a[e] = y;
+        }
+      x[i][0].take(a);
+      x[i][1].take(b);
     }
+    if (!is_q && at < 0) continue;
+    T* to = (is_q ? reinterpret_cast<T*>(p.q_out) + t * p.ot + r * p.oh
+                  : reinterpret_cast<T*>(is_v ? p.v_pages : p.k_pages) + at + int64_t(is_v ? r - n_qk : r - n_q) * p.page_size * p.head_dim) + d;
+    x[i][0].store(to);
+    x[i][1].store(to + half);
   }
 }
 
@@ -200,7 +222,7 @@ template <typename T, int LANES> cudaError_t launch_vec(tl_ctx* ctx, const Appen
   return tl_launch_waiting(kernel, grid, dim3(kThreads), ctx->stream, p);
 }
 template <typename T> cudaError_t launch_lanes(tl_ctx* ctx, const AppendArgs& p, int rows) {
-  if (p.head_dim <= 64) return launch_vec<T, 8>(ctx, p, rows);
+  if (p.head_dim <= 64) return launch_vec<T, 8>(ctx, p, rows);  // a lane: 4 + 4 dimensions
   if (p.head_dim <= 128) return launch_vec<T, 16>(ctx, p, rows);
   return launch_vec<T, 32>(ctx, p, rows);
 }
@@ -258,13 +280,13 @@ int32_t tl_paged_append(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t*
   p.n_seqs = cache->n_seqs; p.max_pages = cache->max_pages; p.dtype = cache->dtype; p.w_dtype = weight_dtype;
   p.eps = eps; p.status = ctx->dev_status + 1;
   const int64_t rows = (q ? n_heads : 0) + 2 * int64_t(cache->n_kv_heads), esz = int64_t(tl_dtype_size(cache->dtype));
-  // Both halves of a head are whole vectors, and every row, weight and table starts on 16 bytes
+  // Both halves of a head are whole vectors of four, and every row, weight and table starts on 16 bytes
   uintptr_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(cache->k_pages) |
                    reinterpret_cast<uintptr_t>(cache->v_pages) | reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight) |
                    reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table) |
                    uintptr_t((k_token_stride | k_head_stride | v_token_stride | v_head_stride) * esz);
   if (q) bits |= reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | uintptr_t((q_token_stride | q_head_stride | out_token_stride | out_head_stride) * esz);
-  if (cache->head_dim % 16 == 0 && cache->head_dim <= 256 && (bits & 15) == 0 && rows <= 65535) {
+  if (cache->head_dim % 8 == 0 && cache->head_dim <= 256 && (bits & 15) == 0 && rows <= 65535) {
     TL_CUDA(ctx, cache->dtype == TL_F32 ? launch_lanes<float>(ctx, p, int(rows))
                                         : cache->dtype == TL_F16 ? launch_lanes<__half>(ctx, p, int(rows)) : launch_lanes<__nv_bfloat16>(ctx, p, int(rows)));
   } else {

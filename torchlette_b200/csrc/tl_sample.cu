@@ -46,7 +46,7 @@ struct SampleArgs {
 using u64 = unsigned long long;
 struct Shared {
   u64 group_max[kGroups];      // (key, ~index) of every group of the cluster
-  u64 told[2][kMaxCluster];    // one value a CTA, two turns
+  u64 told[2][2 * kMaxCluster];  // one or two values a CTA, two turns
   u64 part[kWarps];
   double table[128];           // 2^(j / 128)
   uint32_t count[kBins], mass_low[kBins], mass_high[kBins];  // of this CTA's slice
@@ -76,17 +76,22 @@ template <typename T> struct Row {
   int last;
   Shared* s;
 
-  // f(index, value) for the elements of the slice that are this thread's, eight neighbours at a time
-  template <typename F> __device__ __forceinline__ void each_of(int i, F&& f) const {
+  static constexpr int kLoads = sizeof(T) == 4 ? 2 : 1;
+  struct Eight {
+    uint4 u[kLoads];
+  };
+  __device__ __forceinline__ bool whole(int i) const { return vec && i + 8 <= end; }
+  __device__ __forceinline__ void fetch(int i, Eight& e) const {
+    if (whole(i))
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) e.u[j] = __ldg(reinterpret_cast<const uint4*>(x + i) + j);
+  }
+  template <typename F> __device__ __forceinline__ void take(int i, const Eight& u, F&& f) const {
     if (i >= end) return;
     float v[8];
-    if (vec && i + 8 <= end) {
-      constexpr int kLoads = sizeof(T) == 4 ? 2 : 1;
-      uint4 u[kLoads];
+    if (whole(i)) {
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(x + i) + j);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = clean(DT<T>::to_f32(reinterpret_cast<const T*>(u)[e]));
+      for (int e = 0; e < 8; ++e) v[e] = clean(DT<T>::to_f32(reinterpret_cast<const T*>(u.u)[e]));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = i + e < end ? clean(DT<T>::to_f32(x[i + e])) : -INFINITY;
@@ -94,8 +99,22 @@ template <typename T> struct Row {
 #pragma unroll
     for (int e = 0; e < 8; ++e) f(i + e, v[e]);
   }
+  // f(index, value) for the elements of the slice that are this thread's, eight neighbours at a time
+  template <typename F> __device__ __forceinline__ void each_of(int i, F&& f) const {
+    Eight e;
+    fetch(i, e);
+    take(i, e, f);
+  }
   template <typename F> __device__ __forceinline__ void each(F&& f) const {
-    for (int i = begin + int(threadIdx.x) * 8; i < end; i += kThreads * 8) each_of(i, f);
+    constexpr int kStep = kThreads * 8;
+    Eight now, then;
+    int i = begin + int(threadIdx.x) * 8;
+    fetch(i, now);
+    for (; i < end; i += kStep) {  // the next vector is on its way while this one is looked at
+      fetch(i + kStep, then);
+      take(i, now, f);
+      now = then;
+    }
   }
   __device__ __forceinline__ bool kept(int i, uint32_t key) const { return key > threshold || (key == threshold && i <= last); }
   __device__ __forceinline__ u64 mass_of(float v) const {
@@ -143,10 +162,14 @@ template <typename T> struct Row {
     return v + before;
   }
   // Every CTA's value in s->told[turn]: two turns, so that a CTA may tell the next while another still reads this one
-  __device__ __forceinline__ const u64* tell(u64 v) {
+  __device__ __forceinline__ const u64* tell(u64 v, u64 second = 0) {
     turn ^= 1;
     cg::cluster_group cluster = cg::this_cluster();
-    if (int(threadIdx.x) < ctas) cluster.map_shared_rank(s->told[turn], threadIdx.x)[rank_in] = v;
+    if (int(threadIdx.x) < ctas) {
+      u64* to = cluster.map_shared_rank(s->told[turn], threadIdx.x);
+      to[rank_in] = v;
+      to[kMaxCluster + rank_in] = second;
+    }
     cluster.sync();
     return s->told[turn];
   }
@@ -237,18 +260,38 @@ template <typename T> struct Row {
       uint32_t counts[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) { metric[j] = 0; counts[j] = 0; }
-      if (has)
-        for (int c = 0; c < ctas; ++c) {
-          const uint32_t* rc = cluster.map_shared_rank(s->count, c);
-          const uint32_t* rl = cluster.map_shared_rank(s->mass_low, c);
-          const uint32_t* rh = cluster.map_shared_rank(s->mass_high, c);
+      if (has) {
+        if (per == 1) {  // eight CTAs' at once: a remote load takes as long as a meeting
+          for (int c0 = 0; c0 < ctas; c0 += 8) {
+            uint32_t n[8], lo[8], hi[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < per) {
-              counts[j] += rc[b0 + j];
-              if (MASS) metric[j] += (u64(rh[b0 + j]) << 32) + rl[b0 + j];
+            for (int c = 0; c < 8; ++c) {
+              const bool there = c0 + c < ctas;
+              const int from = there ? c0 + c : 0;
+              n[c] = there ? cluster.map_shared_rank(s->count, from)[b0] : 0u;
+              lo[c] = MASS && there ? cluster.map_shared_rank(s->mass_low, from)[b0] : 0u;
+              hi[c] = MASS && there ? cluster.map_shared_rank(s->mass_high, from)[b0] : 0u;
             }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              counts[0] += n[c];
+              metric[0] += (u64(hi[c]) << 32) + lo[c];
+            }
+          }
+        } else {
+          for (int c = 0; c < ctas; ++c) {
+            const uint32_t* rc = cluster.map_shared_rank(s->count, c);
+            const uint32_t* rl = cluster.map_shared_rank(s->mass_low, c);
+            const uint32_t* rh = cluster.map_shared_rank(s->mass_high, c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < per) {
+                counts[j] += rc[b0 + j];
+                if (MASS) metric[j] += (u64(rh[b0 + j]) << 32) + rl[b0 + j];
+              }
+          }
         }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (!MASS) metric[j] = counts[j];
@@ -277,13 +320,13 @@ template <typename T> struct Row {
       }
       __syncthreads();
       // from the CTA that found it to all
-      const u64* where = tell((u64(s->bin) << 32) | s->bin_count);
+      const u64* where = tell((u64(s->bin) << 32) | s->bin_count, s->above);
       int owner = 0;
       for (int c = 0; c < ctas; ++c)
         if (uint32_t(where[c] >> 32) != 0xffffffffu) owner = c;
       const int bin = int(where[owner] >> 32);
       ties = uint32_t(where[owner]);
-      above = tell(s->above)[owner];
+      above = where[kMaxCluster + owner];
       first = false;
       if (ties <= kCandidates && (linear || shift_of > 0)) {
         // few: ranked by the first CTA
@@ -387,7 +430,7 @@ __device__ __forceinline__ u64 to_reach(double u, u64 whole) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   Shared& s = *reinterpret_cast<Shared*>(dynamic);
   cg::cluster_group cluster = cg::this_cluster();
