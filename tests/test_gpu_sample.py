@@ -172,6 +172,15 @@ def test_rows_apart_and_not_aligned(backend, dtype):
         x.destroy()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_vocabulary_of_millions(backend, dtype):
+    """One row over more than a cluster keeps the masses of, with and without filters."""
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((1, 5_000_001)) * 2
+    for k, p, m in ((None, None, None), ([100], [0.9], None), (None, [0.7], None), ([5000], None, None), (None, None, [0.01])):
+        check(backend, x, dtype, rng.uniform(size=1), [0.9], k, p, m)
+
+
 def test_many_rows_again_and_in_a_graph(backend):
     be = backend
     rng = np.random.default_rng(7)

@@ -26,6 +26,7 @@
 #include <cooperative_groups.h>
 
 #include "tl_common.cuh"
+#include "tl_tma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -86,35 +87,29 @@ template <typename T> struct Row {
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) e.u[j] = __ldg(reinterpret_cast<const uint4*>(x + i) + j);
   }
-  template <typename F> __device__ __forceinline__ void take(int i, const Eight& u, F&& f) const {
+  // CLEAN: NaN is -infinity and -0 is 0; else as stored
+  template <bool CLEAN, typename F> __device__ __forceinline__ void take(int i, const Eight& u, F&& f) const {
     if (i >= end) return;
     float v[8];
     if (whole(i)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = clean(DT<T>::to_f32(reinterpret_cast<const T*>(u.u)[e]));
+      for (int e = 0; e < 8; ++e) v[e] = DT<T>::to_f32(reinterpret_cast<const T*>(u.u)[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = i + e < end ? clean(DT<T>::to_f32(x[i + e])) : -INFINITY;
+      for (int e = 0; e < 8; ++e) v[e] = i + e < end ? DT<T>::to_f32(x[i + e]) : -INFINITY;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f(i + e, v[e]);
+    for (int e = 0; e < 8; ++e) f(i + e, CLEAN ? clean(v[e]) : v[e]);
   }
   // f(index, value) for the elements of the slice that are this thread's, eight neighbours at a time
-  template <typename F> __device__ __forceinline__ void each_of(int i, F&& f) const {
+  template <bool CLEAN = true, typename F> __device__ __forceinline__ void each_of(int i, F&& f) const {
     Eight e;
     fetch(i, e);
-    take(i, e, f);
+    take<CLEAN>(i, e, f);
   }
-  template <typename F> __device__ __forceinline__ void each(F&& f) const {
-    constexpr int kStep = kThreads * 8;
-    Eight now, then;
-    int i = begin + int(threadIdx.x) * 8;
-    fetch(i, now);
-    for (; i < end; i += kStep) {  // the next vector is on its way while this one is looked at
-      fetch(i + kStep, then);
-      take(i, now, f);
-      now = then;
-    }
+  template <bool CLEAN = true, typename F> __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll 2
+    for (int i = begin + int(threadIdx.x) * 8; i < end; i += kThreads * 8) each_of<CLEAN>(i, f);
   }
   __device__ __forceinline__ bool kept(int i, uint32_t key) const { return key > threshold || (key == threshold && i <= last); }
   __device__ __forceinline__ u64 mass_of(float v) const {
@@ -436,6 +431,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank()), row = int(blockIdx.x) / ctas;
   const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 128) s.table[threadIdx.x] = exp2(double(threadIdx.x) * (1.0 / 128));
+  if (threadIdx.x == 0) s.n_cand = 0;
+  tl_pdl_wait();
   Row<T> r;
   r.x = reinterpret_cast<const T*>(p.logits) + int64_t(row) * p.row_stride;
   r.begin = int(min(int64_t(p.vocab), int64_t(rank) * p.per_cta));
@@ -444,19 +442,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
   const float t = p.temperature ? p.temperature[row] : 1.f;
   const bool greedy = !p.uniforms || !(t > 0.f);
   const int k = p.top_k ? p.top_k[row] : 0;
-  if (threadIdx.x < 128) s.table[threadIdx.x] = exp2(double(threadIdx.x) * (1.0 / 128));
-  if (threadIdx.x == 0) s.n_cand = 0;
+  const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
+  float u = p.uniforms ? p.uniforms[row] : 0.f;
+  u = u > 0.f ? fminf(u, 1.f) : 0.f;
 
-  // the largest logit, of 256 groups of them; the smallest finite one
-  u64 best = 0;
-  float least = INFINITY;
-  r.each([&](int i, float v) {
-    const u64 e = (u64(key_of(v)) << 32) | uint32_t(~i);
-    if (i < r.end) {
-      best = best > e ? best : e;
-      if (v > -INFINITY) least = fminf(least, v);
-    }
+  // the largest logit, the lowest index of equal ones, of 256 groups of them (NaN is never larger)
+  float most = -INFINITY;
+  int at = -1;
+  r.template each<false>([&](int i, float v) {
+    if (v > most) { most = v; at = i; }
   });
+  u64 best = at < 0 ? 0 : (u64(key_of(clean(most))) << 32) | uint32_t(~at);
   const int width = 2 * ctas;  // lanes of a group: 256 / ctas groups in a CTA
   for (int o = width >> 1; o > 0; o >>= 1) {
     const u64 e = __shfl_xor_sync(0xffffffffu, best, o);
@@ -486,33 +482,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
   r.threshold = kNone;
   r.last = -1;
   r.min_key = 0;
-  if (p.min_p && p.min_p[row] > 0.f) {
-    const double least_kept = p.min_p[row] < 1.f ? double(r.max) + double(t) * log(double(p.min_p[row])) : double(r.max);
+  if (min_p > 0.f) {
+    const double least_kept = min_p < 1.f ? double(r.max) + double(t) * log(double(min_p)) : double(r.max);
     float f = float(least_kept);
     if (double(f) < least_kept) f = nextafterf(f, INFINITY);
     r.min_key = key_of(clean(f));
   }
-  float u = p.uniforms[row];
-  u = u > 0.f ? fminf(u, 1.f) : 0.f;
-  const float top_p = p.top_p ? p.top_p[row] : 1.f;
 
   if (k > 0 && k <= kMaxQuick && k < p.vocab) {
-    // The k-th largest of the groups' maxima: at least k logits are not below it
-    if (threadIdx.x == 0) s.low = kNone + 1;
-    __syncthreads();
-    {
-      const int g = int(threadIdx.x) >> 1, half = threadIdx.x & 1;
-      const u64 mine = s.group_max[g];
-      int before = 0;
-      for (int j = half * (kGroups / 2); j < (half + 1) * (kGroups / 2); ++j) before += s.group_max[j] > mine;
-      before += __shfl_xor_sync(0xffffffffu, before, 1);
-      if (half == 0 && before == k - 1 && uint32_t(mine >> 32) > kNone) s.low = uint32_t(mine >> 32);
+    // The k-th largest of the groups' maxima, its first 20 bits: at least k logits are not below it.  Bit by bit, by every warp for itself.
+    uint32_t mine[kGroups / 32], from = 0;
+#pragma unroll
+    for (int j = 0; j < kGroups / 32; ++j) mine[j] = uint32_t(s.group_max[j * 32 + lane] >> 32);
+    for (int bit = 31; bit >= 12; --bit) {
+      const uint32_t tried = from | (1u << bit);
+      int above = 0;
+#pragma unroll
+      for (int j = 0; j < kGroups / 32; ++j) above += __popc(__ballot_sync(0xffffffffu, mine[j] >= tried));
+      if (above >= k) from = tried;
     }
-    __syncthreads();
-    const uint32_t from = s.low;
-    r.each([&](int i, float v) {
-      const uint32_t key = key_of(v);
-      if (key >= from) r.send(i, key);
+    from = Row<T>::max_(from, kNone + 1);
+    const float least = of_key(from);
+    r.template each<false>([&](int i, float v) {
+      if (v >= least) r.send(i, key_of(clean(v)));
     });
     cluster.sync();
     const int n = int(*cluster.map_shared_rank(&s.n_cand, 0));
@@ -544,6 +536,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
   }
   if (k > 0 && k < p.vocab) {
     // the smallest finite logit of the row
+    float least = INFINITY;
+    r.each([&](int, float v) { if (v > -INFINITY) least = fminf(least, v); });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
     __syncthreads();
@@ -556,11 +550,53 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
     for (int c = 0; c < ctas; ++c) lo = min(lo, uint32_t(all[c]));
     r.template narrow<false>(u64(k), 0.0, of_key(lo));
   }
-  if (top_p < 1.f) r.template narrow<true>(0, double(fmaxf(top_p, 0.f)), r.max - 31.f * t);
+  if (top_p < 1.f) r.template narrow<true>(0, double(fmaxf(top_p, 0.f)), r.max - 16.f * t);  // what is further behind shares the last bin
   auto weight = [&](int i, float v) -> u64 {
     const uint32_t key = key_of(v);
     return key >= r.min_key && r.kept(i, key) ? r.mass_of(v) : 0ull;
   };
+  const int turns = (p.per_cta + kThreads * 8 - 1) / (kThreads * 8);
+  if (turns * kWarps <= kCandidates) {
+    // The mass of every turn of every warp is kept, so that the CTA with the answer looks at one warp's 256 logits again
+    int turn = 0;
+    u64 mine = 0, before;
+    for (int i = r.begin + int(threadIdx.x) * 8; turn < turns; ++turn, i += kThreads * 8) {
+      u64 w = 0;
+      r.each_of(i, [&](int j, float v) { w += weight(j, v); });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+      if (lane == 0) { s.weight[turn * kWarps + (threadIdx.x >> 5)] = w; mine += w; }
+    }
+    const u64 whole = r.cluster_sum(mine, before), need = to_reach(double(u), whole);
+    const int first = int(threadIdx.x) * 2;
+    const u64 a = first < turns * kWarps ? s.weight[first] : 0, b = first + 1 < turns * kWarps ? s.weight[first + 1] : 0;
+    u64 here;
+    const u64 to = r.block_scan(a + b, here) + before - a - b;
+    if (threadIdx.x == 0) s.n_cand = 0xffffffffu;
+    __syncthreads();
+    if (to < need && to + a >= need) { s.n_cand = first; s.above = to; }
+    if (to + a < need && to + a + b >= need) { s.n_cand = first + 1; s.above = to + a; }
+    __syncthreads();
+    if (threadIdx.x < 32 && s.n_cand != 0xffffffffu) {
+      const int i = r.begin + (int(s.n_cand) / kWarps * kThreads + int(s.n_cand) % kWarps * 32 + lane) * 8;
+      u64 w = 0;
+      r.each_of(i, [&](int j, float v) { w += weight(j, v); });
+      u64 run = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 v = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += v;
+      }
+      run += s.above - w;
+      if (run < need && run + w >= need)
+        r.each_of(i, [&](int j, float v) {
+          const u64 x = weight(j, v);
+          if (run < need && run + x >= need) p.out[row] = j;
+          run += x;
+        });
+    }
+    return;
+  }
   u64 mine = 0, before;
   r.each([&](int i, float v) { mine += weight(i, v); });
   const u64 whole = r.cluster_sum(mine, before);
@@ -604,15 +640,16 @@ int32_t tl_sample(tl_ctx* ctx, const void* logits, int32_t dtype, int64_t rows, 
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1] = tl_pdl_attribute();
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = unsigned(ctas);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   TL_CUDA(ctx, cudaLaunchKernelEx(&cfg, kernel, p));
   ctx->counters[TL_COUNTER_KERNEL_LAUNCHES]++;
-  tl_wrote(ctx, out_tokens, rows * int64_t(sizeof(int32_t)));
+  tl_wrote(ctx, out_tokens, rows * int64_t(sizeof(int32_t)), true);
   return TL_OK;
 }
 
