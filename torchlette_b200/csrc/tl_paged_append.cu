@@ -26,6 +26,7 @@ struct AppendArgs {
   int64_t tokens, table_rows, n_pages;
   int32_t n_heads, n_kv_heads, head_dim, page_size, n_seqs, max_pages, dtype, w_dtype;
   float eps;
+  TlDivide page_div;
   int* status;
 };
 
@@ -36,7 +37,7 @@ __device__ __forceinline__ bool place(const AppendArgs& p, int64_t t, int& pos, 
   const int64_t seq = p.token_seq ? int64_t(p.token_seq[t]) : t;
   const int bad = tl_bad_token(pos, seq, p.n_seqs, p.max_pages, p.page_size, p.cos_t ? p.table_rows : -1);
   if (bad) { atomicOr(p.status, bad); return false; }
-  const int index = pos / p.page_size, page = p.page_table[seq * p.max_pages + index];
+  const int index = tl_divide(pos, p.page_div), page = p.page_table[seq * p.max_pages + index];
   at = -1;
   if (tl_bad_page(page, p.n_pages)) atomicOr(p.status, kBadPage);
   else at = tl_page_at(page, pos - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim);
@@ -108,10 +109,15 @@ template <typename T> struct Four {
     for (int e = 0; e < 4; ++e) v[e] = DT<T>::to_f32(reinterpret_cast<const T*>(&u)[e]);
   }
   __device__ __forceinline__ void take(const float (&v)[4]) {
-    T e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = DT<T>::from_f32(v[i]);
-    u = *reinterpret_cast<const Bits*>(e);
+    if constexpr (std::is_same_v<T, __half>) {
+      const __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
+      u = *reinterpret_cast<const Bits*>(h);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+      u = *reinterpret_cast<const Bits*>(h);
+    } else {
+      u = *reinterpret_cast<const Bits*>(v);
+    }
   }
 };
 __device__ __forceinline__ void load4_any(const void* p, int dtype, int i, float (&v)[4]) {
@@ -128,30 +134,30 @@ __device__ __forceinline__ void load4_any(const void* p, int dtype, int i, float
     f.values(v);
   }
 }
-// A group of LANES lanes (a power of two that holds head_dim / 8) a head, HEADS heads a thread, a CTA for a token's next kThreads / LANES * HEADS heads.  A
+// A group of LANES lanes (a power of two that holds head_dim / 8) a head, HEADS heads a thread, a CTA for a token's next THREADS / LANES * HEADS heads.  A
 // lane has four dimensions of the first half and the same four of the second, which the rotation mixes: no lane needs another's.  The rows are held as
 // stored until their turn, so that several CTAs an SM have loads on their way.  (Eight neighbouring dimensions a lane and shuffles: 52 us for
 // 8001 tokens x 48 heads x 128 bf16, 197 MB, by the instructions that it issued.)
-constexpr int kThreads = 256;
-template <typename T, int LANES, int HEADS>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) append_vec_kernel(const __grid_constant__ AppendArgs p) {
+template <typename T, int LANES, int HEADS, int THREADS>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 1024 / THREADS : 768 / THREADS) append_vec_kernel(const __grid_constant__ AppendArgs p) {
   tl_pdl_wait();
   const int64_t t = blockIdx.x;
+  int pos = p.positions[t];  // asked for before the rows: the page and the rotation wait for it
   const int half = p.head_dim >> 1, d = 4 * int(threadIdx.x % LANES);
   const int n_q = p.q ? p.n_heads : 0, n_qk = n_q + p.n_kv_heads, rows = n_qk + p.n_kv_heads;
-  constexpr int kStep = kThreads / LANES;
+  constexpr int kStep = THREADS / LANES;
   const int first = int(blockIdx.y) * (kStep * HEADS) + int(threadIdx.x) / LANES;
   const bool lane_in = d < half;
 
-  int pos = p.positions[t];  // asked for before the rows: the page and the rotation wait for it
+  // (heads are at most 2^31 elements apart here, so that a head costs no 64-bit product)
+  const T *q = reinterpret_cast<const T*>(p.q) + t * p.qt + d, *k = reinterpret_cast<const T*>(p.k) + t * p.kt + d, *v = reinterpret_cast<const T*>(p.v) + t * p.vt + d;
+  const int qh = int(p.qh), kh = int(p.kh), vh = int(p.vh), oh = int(p.oh), gh = p.page_size * p.head_dim;
   Four<T> x[HEADS][2];
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
     const int r = first + i * kStep;
     if (lane_in && r < rows) {
-      const T* from = (r < n_q ? reinterpret_cast<const T*>(p.q) + t * p.qt + r * p.qh
-                               : r < n_qk ? reinterpret_cast<const T*>(p.k) + t * p.kt + (r - n_q) * p.kh
-                                          : reinterpret_cast<const T*>(p.v) + t * p.vt + (r - n_qk) * p.vh) + d;
+      const T* from = r < n_q ? q + r * qh : r < n_qk ? k + (r - n_q) * kh : v + (r - n_qk) * vh;
       x[i][0].load(from);
       x[i][1].load(from + half);
     }
@@ -163,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) append_vec_k
     load4_any(p.cos_t + int64_t(pos) * half, TL_F32, d, c);
     load4_any(p.sin_t + int64_t(pos) * half, TL_F32, d, s);
   }
+  T *q_out = reinterpret_cast<T*>(p.q_out) + t * p.ot + d, *k_out = reinterpret_cast<T*>(p.k_pages) + at + d, *v_out = reinterpret_cast<T*>(p.v_pages) + at + d;
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
     const int r = first + i * kStep;
@@ -204,22 +211,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) append_vec_k
       x[i][1].take(b);
     }
     if (!is_q && at < 0) continue;
-    T* to = (is_q ? reinterpret_cast<T*>(p.q_out) + t * p.ot + r * p.oh
-                  : reinterpret_cast<T*>(is_v ? p.v_pages : p.k_pages) + at + int64_t(is_v ? r - n_qk : r - n_q) * p.page_size * p.head_dim) + d;
+    T* to = is_q ? q_out + r * oh : is_v ? v_out + (r - n_qk) * gh : k_out + (r - n_q) * gh;
     x[i][0].store(to);
     x[i][1].store(to + half);
   }
 }
 
-// A thread takes one head while the tokens are too few to fill the chip (their loads all at once), else as many as a token's heads ask for, at most
-// four (fewer loads of positions and tables a head).
+// A thread takes one head while the tokens are too few to fill the chip (their loads all at once), else as many of a token's as six, in smaller
+// CTAs: what a thread works out once (its token's place, pages and rotation) costs about as many instructions as two heads (8001 tokens x 48
+// heads x 128 bf16: 47 us with three heads a thread).
+template <typename T, int LANES, int HEADS, int THREADS> cudaError_t launch_heads(tl_ctx* ctx, const AppendArgs& p, int rows) {
+  constexpr int kRows = THREADS / LANES * HEADS;
+  return tl_launch_waiting(append_vec_kernel<T, LANES, HEADS, THREADS>, dim3(unsigned(p.tokens), unsigned((rows + kRows - 1) / kRows)), dim3(THREADS), ctx->stream, p);
+}
 template <typename T, int LANES> cudaError_t launch_vec(tl_ctx* ctx, const AppendArgs& p, int rows) {
-  constexpr int kStep = kThreads / LANES;
-  const int heads = int64_t(p.tokens) * rows < int64_t(ctx->sm_count) * 8 * kStep ? 1 : std::min(4, (rows + kStep - 1) / kStep);
-  const dim3 grid(unsigned(p.tokens), unsigned((rows + kStep * heads - 1) / (kStep * heads)));
-  const auto kernel = heads == 1 ? append_vec_kernel<T, LANES, 1> : heads == 2 ? append_vec_kernel<T, LANES, 2>
-                                 : heads == 3 ? append_vec_kernel<T, LANES, 3> : append_vec_kernel<T, LANES, 4>;
-  return tl_launch_waiting(kernel, grid, dim3(kThreads), ctx->stream, p);
+  if (int64_t(p.tokens) * rows < int64_t(ctx->sm_count) * 8 * (256 / LANES)) return launch_heads<T, LANES, 1, 256>(ctx, p, rows);
+  const int each = (rows + 128 / LANES - 1) / (128 / LANES);  // heads for a thread of a CTA that takes the token whole
+  if (each <= 2) return launch_heads<T, LANES, 2, 128>(ctx, p, rows);
+  if (each <= 4) return launch_heads<T, LANES, 4, 128>(ctx, p, rows);
+  return launch_heads<T, LANES, 6, 128>(ctx, p, rows);
 }
 template <typename T> cudaError_t launch_lanes(tl_ctx* ctx, const AppendArgs& p, int rows) {
   if (p.head_dim <= 64) return launch_vec<T, 8>(ctx, p, rows);  // a lane: 4 + 4 dimensions
@@ -278,15 +288,17 @@ int32_t tl_paged_append(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t*
   p.tokens = tokens; p.table_rows = table_rows; p.n_pages = cache->n_pages;
   p.n_heads = int32_t(n_heads); p.n_kv_heads = cache->n_kv_heads; p.head_dim = cache->head_dim; p.page_size = cache->page_size;
   p.n_seqs = cache->n_seqs; p.max_pages = cache->max_pages; p.dtype = cache->dtype; p.w_dtype = weight_dtype;
+  p.page_div = tl_divide_by(cache->page_size);
   p.eps = eps; p.status = ctx->dev_status + 1;
   const int64_t rows = (q ? n_heads : 0) + 2 * int64_t(cache->n_kv_heads), esz = int64_t(tl_dtype_size(cache->dtype));
+  const int64_t widest = std::max({q_head_stride * (q != nullptr), out_head_stride * (q != nullptr), k_head_stride, v_head_stride, int64_t(cache->page_size) * cache->head_dim});
   // Both halves of a head are whole vectors of four, and every row, weight and table starts on 16 bytes
   uintptr_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(cache->k_pages) |
                    reinterpret_cast<uintptr_t>(cache->v_pages) | reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight) |
                    reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table) |
                    uintptr_t((k_token_stride | k_head_stride | v_token_stride | v_head_stride) * esz);
   if (q) bits |= reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | uintptr_t((q_token_stride | q_head_stride | out_token_stride | out_head_stride) * esz);
-  if (cache->head_dim % 8 == 0 && cache->head_dim <= 256 && (bits & 15) == 0 && rows <= 65535) {
+  if (cache->head_dim % 8 == 0 && cache->head_dim <= 256 && (bits & 15) == 0 && rows <= 65535 && rows * widest <= INT32_MAX) {
     TL_CUDA(ctx, cache->dtype == TL_F32 ? launch_lanes<float>(ctx, p, int(rows))
                                         : cache->dtype == TL_F16 ? launch_lanes<__half>(ctx, p, int(rows)) : launch_lanes<__nv_bfloat16>(ctx, p, int(rows)));
   } else {
