@@ -337,9 +337,9 @@ TL_API int32_t tl_decode_attention(tl_ctx* ctx, const void* q, const void* k_cac
  * positions[t] is the position of token t in its sequence and token_seq[t] that sequence (NULL: token t belongs to sequence t).
  * A negative position marks a token that is not there (a padded batch): nothing of it is read or written, only tl_paged_attention
  * writes zeros for it.  positions, token_seq and page_table are int32 on the device, read when the kernel runs, so that a captured step replays
- * with new ones.  What only the kernel can see -- a position past max_pages * page_size or the rotation tables, a
- * sequence or page that is not there -- skips that token (a page of the past: those keys), touches no memory, and is reported by the next
- * tl_sync as TL_ERR_INVALID_ARG. */
+ * with new ones.  What only the kernel can see is skipped, touches no memory, and is reported by the next tl_sync as TL_ERR_INVALID_ARG:
+ * a token whose position lies past max_pages * page_size (tl_paged_append: or the rotation tables) or whose sequence is not there, as if its position
+ * were negative; of a page that is not there, the keys and values that would be stored in it or read from it. */
 typedef struct tl_paged_cache {
   void* k_pages;
   void* v_pages;
@@ -356,8 +356,8 @@ typedef struct tl_paged_cache {
  * each token's position (where the tables are given, f32 [table_rows, head_dim / 2]) and the append of k and v, one launch.
  * q [tokens, n_heads, head_dim], k and v [tokens, n_kv_heads, head_dim] with any strides in elements between tokens and between heads
  * (the columns of one fused product, or the [heads, tokens, head_dim] order of tl_rope); q_out likewise.  q may be NULL
- * (k and v alone) and q_out may be q itself with q's strides.  Two tokens of a call at the same position of a sequence leave
- * that position undefined.  head_dim is even, at most 1024. */
+ * (k and v alone) and q_out may be q itself with q's strides; no other output overlaps an input.  Two tokens of a call at the same position of a
+ * sequence leave that position undefined.  head_dim is even, at most 1024. */
 TL_API int32_t tl_paged_append(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t* positions, const int32_t* token_seq, int64_t tokens,
                                const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t n_heads, void* q_out,
                                int64_t out_token_stride, int64_t out_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride,
@@ -369,7 +369,8 @@ TL_API int32_t tl_paged_append(tl_ctx* ctx, const tl_paged_cache* cache, const i
  *   x_j = q . k_j * scale;  softcap > 0: x_j = softcap * tanh(x_j / softcap);  slopes: x_j += slopes[h] * (j - p)  (f32 [n_heads])
  *   out = sum_j softmax(x)_j v_j, zeros where nothing is seen.
  * Several tokens of one sequence in a call are rows of their own (each reads the cache).  head_dim is a multiple of 8, at most 256;
- * pages, q and out start on 16 bytes and the strides are multiples of 16 bytes. */
+ * pages, q and out start on 16 bytes and the strides are multiples of 16 bytes.  softcap is 0 or at least 1e-30.  The context's calls share a
+ * scratch of fixed size, made by the first call (a call in a graph capture before it is refused): captured calls, too, are replayed one after another. */
 TL_API int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t* positions, const int32_t* token_seq, int64_t tokens,
                                   const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t n_heads, void* out, float scale,
                                   float softcap, int32_t window, const float* slopes);

@@ -336,27 +336,28 @@ def test_attention_reads_strided_queries(backend):
     assert_close(out, ref, slack, "bf16")
 
 
-def test_indexes_out_of_range_are_skipped_and_reported():
+@pytest.mark.parametrize("page", [16, 5])
+def test_indexes_out_of_range_are_skipped_and_reported(page):
     """Positions, sequences and pages that are not there: no memory is touched, the other tokens are right, the next sync says so, once."""
     be = tb.CudaBackend(0)  # its error count is its own
     try:
-        _out_of_range(be)
+        _out_of_range(be, page)
     finally:
         be.destroy()
 
 
-def _out_of_range(be):
+def _out_of_range(be, page_size):
     gen = torch.Generator(device="cuda").manual_seed(6)
-    c = Cache(be, gen, [40, 40, 40, 40], 2, 64, 16, "f16")
+    c = Cache(be, gen, [40, 40, 40, 40], 2, 64, page_size, "f16")
     for i in range(4):
         c.fill(gen, i, 40, "f16")
-    room = c.table.shape[1] * 16
+    room = c.table.shape[1] * page_size
     q, k, v = (normal(gen, (4, n, 64), "f16") for n in (4, 2, 2))
     cos = torch.ones(60, 32, device="cuda")
     errors = be.getGpuUncapturedErrorCount()
     for pos, seq, word in (([39, room, 5, 39], [0, 1, 2, 3], "position"), ([39, 2 ** 31 - 1, 5, 39], [0, 1, 2, 3], "position"),
                            ([39, 5, 5, 39], [0, 4, 2, 3], "sequence"), ([39, 5, 5, 39], [0, -1, 2, 3], "sequence"),
-                           ([39, 50, 5, 39], [0, 1, 2, 3], "page")):  # 50: the table's junk
+                           ([39, room - 1, 5, 39], [0, 1, 2, 3], "page")):  # the last page of the table is junk
         p, s = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (pos, seq))
         before = c.k.clone(), c.v.clone()
         out = torch.full((4, 4, 64), 7.0, device="cuda", dtype=torch.float16)
@@ -387,6 +388,93 @@ def _out_of_range(be):
         if word != "page":
             assert (y[1] == 0).all()
     assert be.getGpuUncapturedErrorCount() == errors + 10
+
+
+def test_a_page_of_the_past_that_is_not_there(backend_of_its_own):
+    """Its keys do not count, the others do: the same as attention over them alone."""
+    be = backend_of_its_own
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    for page_size, dtype in ((16, "bf16"), (7, "bf16"), (8, "f32")):
+        c = Cache(be, gen, [100], 2, 64, page_size, dtype)
+        c.fill(gen, 0, 100, dtype)
+        q, pos = normal(gen, (1, 4, 64), dtype), torch.tensor([99], dtype=torch.int32, device="cuda")
+        c.table[0, 2] = JUNK
+        out = torch.empty(1, 256, device="cuda", dtype=TORCH[dtype])
+        torch.cuda.synchronize()
+        be.ops.pagedAttention(c.cache, wrap(be, pos), wrap(be, q), 0.125, out=wrap(be, out))
+        with pytest.raises(tb.TlError, match="page"):
+            be.sync()
+        at = torch.cat([torch.arange(2 * page_size), torch.arange(3 * page_size, 100)]).cuda()
+        k, v = (x[c.table[0, at // page_size].long(), :, at % page_size].double().repeat_interleave(2, 1) for x in (c.k, c.v))
+        w = torch.softmax(torch.einsum("hd,jhd->hj", q[0].double(), k) * 0.125, 1)
+        ref = torch.einsum("hj,jhd->hd", w, v)
+        assert_close(out.view(4, 64), ref, torch.full_like(ref, 2e-4), dtype)
+        c.table[:] = JUNK  # none is there
+        torch.cuda.synchronize()
+        be.ops.pagedAttention(c.cache, wrap(be, pos), wrap(be, q), 0.125, out=wrap(be, out))
+        with pytest.raises(tb.TlError, match="page"):
+            be.sync()
+        assert (out == 0).all()
+
+
+@pytest.fixture
+def backend_of_its_own():
+    be = tb.CudaBackend(0)  # its error count and scratch are its own
+    yield be
+    be.destroy()
+
+
+def test_a_first_call_in_a_capture_is_refused(backend_of_its_own):
+    be = backend_of_its_own
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    c = Cache(be, gen, [20], 1, 64, 16, "f16")
+    c.fill(gen, 0, 20, "f16")
+    q, pos, out = normal(gen, (1, 2, 64), "f16"), torch.tensor([19], dtype=torch.int32, device="cuda"), torch.zeros(1, 128, device="cuda", dtype=torch.float16)
+    torch.cuda.synchronize()
+    call = lambda: be.ops.pagedAttention(c.cache, wrap(be, pos), wrap(be, q), 0.125, out=wrap(be, out))  # noqa: E731
+    be.beginCapture()
+    with pytest.raises(tb.TlError, match="before capturing") as e:
+        call()
+    assert e.value.status == B.TL_ERR_UNSUPPORTED
+    be.destroyGraph(be.endCapture())
+    call()
+    be.sync()
+    be.beginCapture()
+    call()
+    graph = be.endCapture()
+    out.zero_()
+    torch.cuda.synchronize()
+    be.replay(graph)
+    be.sync()
+    ref, slack = attention_ref(c, q, pos, [0], 0.125)
+    assert_close(out.view(1, 2, 64), ref, slack, "f16")
+    be.destroyGraph(graph)
+
+
+@pytest.mark.parametrize("page", [16, 6])
+def test_a_cache_past_32_bits(backend, page):
+    """Pages behind the 2^31st element, and the 2^32nd byte: append there and attention over it."""
+    be, g, d = backend, 8, 128
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    pages = 2 ** 31 // (g * page * d) + 40
+    k, v = (torch.empty(pages, g, page, d, device="cuda", dtype=torch.float16) for _ in range(2))
+    n = 5 * page + 3
+    table = torch.arange(pages - 1, pages - 7, -1, dtype=torch.int32, device="cuda")[None].contiguous()
+    tensors = [wrap(be, k), wrap(be, v), wrap(be, table)]
+    cache = be.createPagedCache(*tensors)
+    kn, vn, q = normal(gen, (n, g, d), "f16"), normal(gen, (n, g, d), "f16"), normal(gen, (1, 16, d), "f16")
+    pos, seq = torch.arange(n, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    be.ops.pagedAppend(cache, wrap(be, pos), None, wrap(be, kn), wrap(be, vn), tokenSeq=wrap(be, seq))
+    out = be.ops.pagedAttention(cache, wrap(be, pos[-1:]), wrap(be, q), 0.09)
+    be.sync()
+    at = torch.arange(n, device="cuda")
+    assert torch.equal(k[table[0, at // page].long(), :, at % page], kn) and torch.equal(v[table[0, at // page].long(), :, at % page], vn)
+    w = torch.softmax(torch.einsum("hd,jhd->hj", q[0].double(), kn.double().repeat_interleave(2, 1)) * 0.09, 1)
+    ref = torch.einsum("hj,jhd->hd", w, vn.double().repeat_interleave(2, 1))
+    got = torch.from_numpy(np.float64(be.ops.read(out))).cuda().view(16, d)
+    assert_close(got, ref, torch.full_like(ref, 1e-4), "f16")
+    out.destroy()
 
 
 def test_a_captured_step_replays_with_new_positions(backend):

@@ -100,6 +100,7 @@ ATTEND = dict(positions=AT, token_seq=None, tokens=3, q=AT, q_ts=256, q_hs=64, h
     ({}, dict(scale=float("nan")), B.TL_ERR_INVALID_ARG, b"finite"),
     ({}, dict(softcap=-1.0), B.TL_ERR_INVALID_ARG, b"softcap"),
     ({}, dict(softcap=float("inf")), B.TL_ERR_INVALID_ARG, b"finite"),
+    ({}, dict(softcap=1e-40), B.TL_ERR_INVALID_ARG, b"1e-30"),
     ({}, dict(window=-3), B.TL_ERR_INVALID_ARG, b"window"),
 ])
 def test_attention_refuses(ctx, cache, args, status, text):

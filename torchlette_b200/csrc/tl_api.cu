@@ -189,6 +189,7 @@ int32_t tl_sync(tl_ctx* ctx) {
     if (ctx->zscratch) cudaMemset(ctx->zscratch, 0, ctx->zscratch_bytes);
     for (auto& p : ctx->retired_scratch) cudaMemset(p.first, 0, p.second);  // older graphs' meeting points too
     if (ctx->stream_scratch) cudaMemset(ctx->stream_scratch, 0, size_t(ctx->sm_count) * (2 * 2 * 128 * sizeof(float) + sizeof(unsigned)));
+    if (ctx->paged_scratch) cudaMemset(ctx->paged_scratch, 0, ctx->paged_scratch_bytes);
     ctx->async_errors++;
     return tl_set_error(ctx, TL_ERR_TIMEOUT, "tl_sync: a kernel gave up a bounded wait (device code %d)", status);
   }

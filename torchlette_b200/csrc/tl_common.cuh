@@ -69,6 +69,7 @@ struct tl_ctx {
   int pf_next = 0;
   int pf_last_grid = 0;
   void* stream_scratch = nullptr;
+  size_t paged_scratch_bytes = 0;
   void* paged_scratch = nullptr;  // where the parts of tokens of tl_paged_attention meet; fixed size, allocated once
   int wait_limit_polls = 1 << 26;  // bound of one device-side wait of the peer collectives
   int push_poll_ranks = 4;         // reduce-on-read: ranks polled together (1 = one after the other)

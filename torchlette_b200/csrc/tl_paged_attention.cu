@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     };
     Batch now = look_up();
     int stage = 0, lap = 0, issued = 0;
-    const int boxes = 2 * ((p.head_dim * int(sizeof(AT)) + 127) / 128), at_once = min(4, 32 / boxes), my_tile = lane / boxes, my_box = lane % boxes;
+    const int boxes = 2 * ((p.head_dim * int(sizeof(AT)) + 127) / 128), at_once = min(min(4, 32 / boxes), p.stages), my_tile = lane / boxes, my_box = lane % boxes;
     bool ok = true;
     while (now.n > 0 && ok) {
       const Batch then = look_up();
@@ -1086,6 +1086,7 @@ int32_t secure_scratch(tl_ctx* ctx) {
     return tl_set_error(ctx, TL_ERR_OOM, "tl_paged_attention: scratch of %zu bytes failed: %s", bytes, cudaGetErrorString(e));
   }
   ctx->paged_scratch = at;
+  ctx->paged_scratch_bytes = bytes;
   TL_CUDA(ctx, cudaMemsetAsync(at, 0, bytes, ctx->stream));
   return TL_OK;
 }
@@ -1104,8 +1105,8 @@ int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32
     return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_attention: %lld heads over %d kv heads", (long long)n_heads, cache->n_kv_heads);
   if (cache->head_dim % 8 != 0 || cache->head_dim > 256)
     return tl_set_error(ctx, TL_ERR_UNSUPPORTED, "tl_paged_attention: head_dim must be a multiple of 8 and at most 256, got %d", cache->head_dim);
-  if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.f || window < 0)
-    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_attention: scale and softcap must be finite, softcap and window not negative");
+  if (!std::isfinite(scale) || !std::isfinite(softcap) || (softcap != 0.f && softcap < 1e-30f) || window < 0)
+    return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_attention: scale and softcap must be finite, softcap 0 or at least 1e-30, window not negative");
   if (tokens == 0) return TL_OK;
   if (!q || !out) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_attention: null pointer");
   const int64_t esz = int64_t(tl_dtype_size(cache->dtype));
