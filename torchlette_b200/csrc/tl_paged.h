@@ -30,6 +30,8 @@ TL_HD int64_t tl_page_at(int32_t page, int32_t slot, int32_t n_kv_heads, int32_t
 // part costs by itself (its queries, the meeting of the warps, its output); so a part of n tiles takes up kLead + n units, the lead first.
 // The units of a call, part after part, are dealt out to `ctas` CTAs in equal contiguous shares.  A share may begin and end inside a
 // part's tiles: what its CTAs make of it meets in scratch.
+// (Without a lead, 64 ragged sequences up to 8000: 160 us against 137, the CTAs with many short ones ending last; 3, 6 and 9 are alike since cuts meet at the
+// end of a share, but f32 shares of few tiles: 14.4 us with 3, 11.6 with 6 and 9.)
 constexpr int kLead = 6;
 TL_HD int32_t tl_tiles(int32_t first_key, int32_t end_key, int32_t keys) {
   return end_key > first_key ? (end_key - 1) / keys + 1 - first_key / keys : 0;
