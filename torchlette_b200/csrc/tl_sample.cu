@@ -629,7 +629,8 @@ int32_t tl_sample(tl_ctx* ctx, const void* logits, int32_t dtype, int64_t rows, 
   p.vocab = int32_t(vocab);
   p.shift = 44;
   while (p.shift > 38 && (vocab >> (62 - p.shift)) != 0) --p.shift;  // the whole mass stays below 2^63
-  // CTAs of a row: as many as keep all rows in one wave of two CTAs an SM, each with a vector a thread
+  // CTAs of a row: as many as keep all rows in one wave of two CTAs an SM, each with a vector a thread; top-p over 151 936 logits with 16 against 8: 16 rows
+  // 45 and 53 us, one row 35 and 44
   int ctas = 1;
   while (ctas < kMaxCluster && vocab > int64_t(ctas) * kThreads * 8 && rows * ctas * 2 <= 2 * int64_t(ctx->sm_count)) ctas *= 2;
   p.per_cta = int32_t(((vocab + ctas - 1) / ctas + 7) / 8 * 8);
