@@ -21,7 +21,8 @@
 // about three times as many.
 //
 // Measured: 64 rows x 151 936 f32, top-k 50 and top-p .95: 25.3 us (39 MB: 6 us of HBM, the rest is the cluster's meetings and the first CTA's ranking);
-// 16 such rows in f16, top-p .9 and min-p .02: 45 us, its passes of 64-bit exponentials over L2 and the meetings between them.
+// 16 such rows in f16, top-p .9 and min-p .02: 45 us, 8 of them the pass into bins (exponentials and shared atomics), 4 each the pass
+// that sends a bin's tokens and the one over the kept masses, the rest meetings and reads of other CTAs' bins.
 #include <algorithm>
 #include <climits>
 #include <cmath>
