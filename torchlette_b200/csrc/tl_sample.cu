@@ -437,6 +437,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 128) s.table[threadIdx.x] = exp2(double(threadIdx.x) * (1.0 / 128));
   if (threadIdx.x == 0) s.n_cand = 0;
+  // All CTAs of the cluster run before one of them writes to another's shared memory: said here, waited for behind the first pass
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   tl_pdl_wait();
   Row<T> r;
   r.x = reinterpret_cast<const T*>(p.logits) + int64_t(row) * p.row_stride;
@@ -462,6 +464,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs p) {
     const u64 e = __shfl_xor_sync(0xffffffffu, best, o);
     best = best > e ? best : e;
   }
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   {
     const int groups = kGroups / ctas, group = int(threadIdx.x) / width;
     for (int c = lane & (width - 1); c < ctas; c += width) cluster.map_shared_rank(s.group_max, c)[rank * groups + group] = best;
