@@ -31,18 +31,20 @@ struct AppendArgs {
   int* status;
 };
 
-// Where token t goes: false if it is not there.  `at`: its element offset in k_pages and v_pages, of head 0, or -1 if its page is not there.
-__device__ __forceinline__ bool place(const AppendArgs& p, int64_t t, int& pos, int64_t& at) {
+// Whether token t is there: nothing but its position and sequence is read of one that is not
+__device__ __forceinline__ bool is_there(const AppendArgs& p, int64_t t, int& pos, int64_t& seq) {
   pos = p.positions[t];
   if (pos < 0) return false;
-  const int64_t seq = p.token_seq ? int64_t(p.token_seq[t]) : t;
+  seq = p.token_seq ? int64_t(p.token_seq[t]) : t;
   const int bad = tl_bad_token(pos, seq, p.n_seqs, p.max_pages, p.page_size, p.cos_t ? p.table_rows : -1);
-  if (bad) { atomicOr(p.status, bad); return false; }
-  const int index = tl_divide(pos, p.page_div), page = p.page_table[seq * p.max_pages + index];
-  at = -1;
-  if (tl_bad_page(page, p.n_pages)) atomicOr(p.status, kBadPage);
-  else at = tl_page_at(page, pos - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim);
-  return true;
+  if (bad) atomicOr(p.status, bad);
+  return !bad;
+}
+// Where it goes: the element offset in k_pages and v_pages of head 0, or -1 if its page is not there.  index: of the page in its sequence
+__device__ __forceinline__ int64_t place(const AppendArgs& p, int pos, int index, int page) {
+  if (!tl_bad_page(page, p.n_pages)) return tl_page_at(page, pos - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim);
+  atomicOr(p.status, kBadPage);
+  return -1;
 }
 
 // Any strides and even head_dim: a warp per token and head (q's, then k's, then v's), a lane per pair of dimensions.
@@ -54,8 +56,10 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs p) {
   for (int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5); w < all; w += step) {
     const int64_t t = w / rows;
     int r = int(w - t * rows), pos;
-    int64_t at;
-    if (!place(p, t, pos, at)) continue;
+    int64_t seq;
+    if (!is_there(p, t, pos, seq)) continue;
+    const int index = tl_divide(pos, p.page_div);
+    const int64_t at = place(p, pos, index, p.page_table[seq * p.max_pages + index]);
     const void *x, *weight;
     void* y;
     int64_t xi, yi;
@@ -143,7 +147,10 @@ template <typename T, int LANES, int HEADS, int THREADS>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 1024 / THREADS : 768 / THREADS) append_vec_kernel(const __grid_constant__ AppendArgs p) {
   tl_pdl_wait();
   const int64_t t = blockIdx.x;
-  int pos = p.positions[t];  // asked for before the rows: the page and the rotation wait for it
+  int pos;
+  int64_t seq;
+  if (!is_there(p, t, pos, seq)) return;  // the same in all threads
+  const int index = tl_divide(pos, p.page_div), page = p.page_table[seq * p.max_pages + index];  // on its way with the rows
   const int half = p.head_dim >> 1, d = 4 * int(threadIdx.x % LANES);
   const int n_q = p.q ? p.n_heads : 0, n_qk = n_q + p.n_kv_heads, rows = n_qk + p.n_kv_heads;
   constexpr int kStep = THREADS / LANES;
@@ -163,8 +170,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 1024 / THREADS : 768
       x[i][1].load(from + half);
     }
   }
-  int64_t at;
-  if (!place(p, t, pos, at)) return;  // the same in all threads
+  const int64_t at = place(p, pos, index, page);
   float c[4], s[4];
   if (lane_in && p.cos_t) {
     load4_any(p.cos_t + int64_t(pos) * half, TL_F32, d, c);
