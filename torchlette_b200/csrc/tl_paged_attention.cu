@@ -143,40 +143,6 @@ struct Cursor {
   template <int KEYS> __device__ __forceinline__ int first_key(int i) const { return (k.lo / KEYS + i) * KEYS; }
 };
 
-// One row again, by one warp and over exactly the keys that it sees: its result is not finite, and whether that is what the cache holds or an infinite value times
-// a probability's low term (zero, or negative) only whole probabilities tell.  Two passes; dimensions d0 .. d0 + 31 are stored.
-template <typename AT>
-__device__ __noinline__ void row_again(const PagedArgs& p, const Token& k, int pos, int t, int h, int kvh, int d0) {
-  const int lane = threadIdx.x & 31;
-  const AT* q = reinterpret_cast<const AT*>(p.q) + int64_t(t) * p.qt + int64_t(h) * p.qh;
-  float mx = -FLT_MAX, sum = 0.f, o = 0.f;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll 1
-    for (int j = k.lo; j < k.hi; ++j) {
-      const int index = tl_divide(j, p.page_div), page = p.page_table[int64_t(k.seq) * p.max_pages + index];
-      if (tl_bad_page(page, p.n_pages)) continue;
-      const int64_t at = tl_page_at(page, j - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim) + int64_t(kvh) * p.page_size * p.head_dim;
-      const AT* kp = reinterpret_cast<const AT*>(p.k_pages) + at;
-      float x = 0.f;
-      for (int d = lane; d < p.head_dim; d += 32) x = fmaf(DT<AT>::to_f32(q[d]), DT<AT>::to_f32(kp[d]), x);
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-      x *= p.scale;
-      if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-      if (p.slopes) x = fmaf(p.slopes[h], float(j - pos), x);
-      if (pass == 0) {
-        mx = fmaxf(mx, x);
-      } else {
-        const float e = expf(x - mx);
-        sum += e;
-        if (d0 + lane < p.head_dim) o = fmaf(e, DT<AT>::to_f32(reinterpret_cast<const AT*>(p.v_pages)[at + d0 + lane]), o);
-      }
-    }
-  }
-  if (d0 + lane < p.head_dim) reinterpret_cast<AT*>(p.out)[(int64_t(t) * p.n_heads + h) * p.head_dim + d0 + lane] = DT<AT>::from_f32(o / sum);
-}
-
 // c tanh(x / c), within a few 2^-23 of itself whatever c is.  From |x / c| = 1/4 on it is c (1 - 2 / (1 + exp(2 x / c))), scale = 2 log2(e) / c, whose error is a
 // few 2^-23 of c, as the value is; below, where that form cancels and a large cap would take the scores with it, x times the first five terms of tanh(y) / y
 // (the sixth is below 2^-26 there).  (16 sequences x <= 6000 keys x 256: 32.5 us, without the near form 32.0; tanhf's two branches were
@@ -189,6 +155,72 @@ __device__ __forceinline__ float cap(float x, float c, float inv, float scale) {
   return fabsf(y) < .25f ? near : far;
 }
 
+// Infinite values and the terms of a probability: one that is zero or negative makes NaN of an infinity.  A NaN of this kind, which no conversion makes, is stored where
+// an output is NaN and the sum of its row's probabilities is not, and look_again() finds it there.
+constexpr uint16_t kUnsettled = 0xfff1;
+template <typename AT> __device__ __forceinline__ bool unsettled(const AT& x) { return reinterpret_cast<const uint16_t&>(x) == kUnsettled; }
+// The part's outputs that are not settled, by all threads of the CTA: what the row sees in that dimension decides.  One infinity is infinity, both, a NaN, and an infinity
+// whose score is -infinity are NaN.  found: [rows][DPAD] words.
+template <typename AT, int DPAD, int THREADS>
+__device__ __noinline__ void look_again(const PagedArgs& p, const Token& k, int t, int kvh, int h0, int rows, uint32_t* found) {
+  constexpr int kAhead = 4;
+  enum { kUp = 1, kDown = 2, kNan = 4 };
+  const int lane = threadIdx.x & 31, d0 = 8 * lane, all = rows * p.head_dim;
+  AT* out = reinterpret_cast<AT*>(p.out) + (int64_t(t) * p.n_heads + h0) * p.head_dim;
+  bool any = false;
+  for (int i = threadIdx.x; i < all; i += THREADS) any |= unsettled(out[i]);
+  for (int i = threadIdx.x; i < rows * DPAD; i += THREADS) found[i] = 0;
+  if (!__syncthreads_or(any)) return;
+  for (int j0 = k.lo + kAhead * (int(threadIdx.x) >> 5); j0 < k.hi; j0 += kAhead * (THREADS / 32)) {
+    int64_t at[kAhead];
+    uint4 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = min(j0 + i, k.hi - 1), index = tl_divide(j, p.page_div), page = p.page_table[int64_t(k.seq) * p.max_pages + index];
+      at[i] = tl_bad_page(page, p.n_pages) || j0 + i >= k.hi ? -1 : tl_page_at(page, j - index * p.page_size, p.n_kv_heads, p.page_size, p.head_dim) + int64_t(kvh) * p.page_size * p.head_dim + d0;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (at[i] >= 0 && d0 < p.head_dim) v[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const AT*>(p.v_pages) + at[i]);
+    }
+#pragma unroll 1
+    for (int i = 0; i < kAhead; ++i) {
+      const AT* e = reinterpret_cast<const AT*>(&v[i]);
+      uint32_t kind = 0;  // three bits for each of the eight
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const float x = DT<AT>::to_f32(e[d]);
+        kind |= uint32_t(isfinite(x) ? 0 : x != x ? kNan : x > 0.f ? kUp : kDown) << (3 * d);
+      }
+      if (!__any_sync(0xffffffffu, kind != 0)) continue;
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) {
+        float x = 0.f;
+        if (d0 < p.head_dim) {
+          const AT *q = reinterpret_cast<const AT*>(p.q) + int64_t(t) * p.qt + int64_t(h0 + r) * p.qh + d0, *kp = reinterpret_cast<const AT*>(p.k_pages) + at[i];
+#pragma unroll
+          for (int d = 0; d < 8; ++d) x = fmaf(DT<AT>::to_f32(q[d]), DT<AT>::to_f32(kp[d]), x);
+        }
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+        x *= p.scale;
+        if (p.softcap > 0.f) x = cap(x, p.softcap, p.cap_inv, p.cap_exp);
+        if (p.slopes) x = fmaf(p.slopes[h0 + r], float(int(j0 + i + 1) - k.hi), x);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const uint32_t is = (kind >> (3 * d)) & 7;
+          if (is) atomicOr(&found[r * DPAD + d0 + d], x == -INFINITY ? uint32_t(kNan) : is);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < all; i += THREADS) {
+    const int r = i / p.head_dim;
+    const uint32_t is = found[r * DPAD + i - r * p.head_dim];
+    if (unsettled(out[i])) out[i] = DT<AT>::from_f32(is == kUp ? INFINITY : is == kDown ? -INFINITY : NAN);
+  }
+  __syncthreads();
+}
+
 // Probabilities are held times 2^10 in f16: the low term of their split stays clear of f16's subnormals.
 template <typename AT> constexpr float kProbBias = 0.f;
 template <> constexpr float kProbBias<__half> = 10.f;
@@ -199,7 +231,7 @@ template <typename AT_, int DPAD_, int NT>
 struct MmaTile {
   using AT = AT_;
   static constexpr int DPAD = DPAD_, ROWS = 8 * NT, KEYS = 16, TERMS = ProbSplit<AT>::kTerms, CTAS = kCtas, WARPS = kConsumerWarps;
-  static constexpr bool kRedo = true;  // infinite values need it
+  static constexpr bool kLookAgain = true;  // infinite values need it: terms of probabilities
   uint32_t q[NT][DPAD / 16][2];
   float o[NT][DPAD / 16][4], m[NT][2], l[NT][2], slope[NT][2];
 
@@ -349,7 +381,7 @@ struct MmaTile {
         }
       }
   }
-  // The rows' outputs straight from the registers, where the warp's keys are all there are; true if one of this lane's is not finite
+  // The rows' outputs straight from the registers, where the warp's keys are all there are; true if one of this lane's is not settled
   __device__ __forceinline__ bool finish(AT* out, int dim, int rows) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     bool odd = false;
@@ -364,12 +396,18 @@ struct MmaTile {
         const float inv = v == 0.f ? 0.f : 1.f / v;
         const int r = nt * 8 + 2 * c + e;
         if (r < rows) {
+          float none = 0.f;  // NaN if one of them is not finite
 #pragma unroll
           for (int i = 0; i < DPAD / 8; ++i) {
             const float x = o[nt][i >> 1][e + 2 * (i & 1)] * inv;
-            if (8 * i < dim) {
-              out[r * dim + 8 * i + g] = DT<AT>::from_f32(x);
-              odd |= !isfinite(x);
+            if (8 * i < dim) out[r * dim + 8 * i + g] = DT<AT>::from_f32(x);
+            none = fmaf(x, 0.f, none);
+          }
+          if (none != none && v > 0.f) {
+#pragma unroll 1
+            for (int d = g; d < dim; d += 8) {
+              const float x = DT<AT>::to_f32(out[r * dim + d]);
+              if (x != x) { reinterpret_cast<uint16_t*>(out)[r * dim + d] = kUnsettled; odd = true; }
             }
           }
         }
@@ -399,7 +437,7 @@ template <int DPAD_, int ROWS_>
 struct F32Tile {
   using AT = float;
   static constexpr int DPAD = DPAD_, ROWS = ROWS_, KEYS = 8, E = DPAD / 32, CTAS = kCtas, WARPS = kConsumerWarps;
-  static constexpr bool kRedo = false;
+  static constexpr bool kLookAgain = false;
   static constexpr int kSets = ROWS * KEYS > 32 ? ROWS * KEYS / 32 : 1, kN = ROWS * KEYS / kSets;  // kN values are summed at once
   static constexpr int kRowsOfSet = ROWS / kSets, kLog = kN == 32 ? 5 : kN == 16 ? 4 : 3;
   float q[ROWS][E], o[ROWS][E];
@@ -639,11 +677,11 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     long long tile0;
     int left;  // in a slot: other CTAs have tiles of it too
   };
-  __shared__ Part cut[2];
+  __shared__ Part first, cut[2];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
   __shared__ uint32_t seen_of[kMaxStages];
   __shared__ long long found_begin, scan[kThreads / 32];
-  __shared__ int found_token, is_last[2], groups_done, abort_flag;
+  __shared__ int found_token, is_last[2], groups_done, any_unsettled, abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = int(blockIdx.x);
   if (int(threadIdx.x) < p.stages) {
     mbar_init(&full[threadIdx.x], TMA ? 1 : 33);  // cp.async: every lane's copies, and the word of what is seen
@@ -652,7 +690,7 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     mbar_fence_init();
   }
   if (threadIdx.x == 0) {
-    abort_flag = is_last[0] = is_last[1] = cut[0].left = cut[1].left = 0;
+    any_unsettled = abort_flag = is_last[0] = is_last[1] = cut[0].left = cut[1].left = 0;
     if (TMA) { tma_prefetch_desc(&k_map); tma_prefetch_desc(&v_map); }
   }
   if (p.head_dim < DPAD) {  // no copy writes the padding: it is zero from here on
@@ -751,6 +789,7 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     return true;
   };
   clip();
+  if (Tile::kLookAgain && threadIdx.x == 0) first = Part{c.t, c.kvh, c.tile, c.n, c.k, tile0, 0};
 
   if (warp == WARPS) {
     // ---- the producer.  A lane looks up a tile's page (cp.async: a row's) a batch before it is copied, so that the table is read on the way.
@@ -850,33 +889,31 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
   // Four neighbouring values of a row by each thread
   auto store = [&](const Part& w, int h0, int e, float4 o, float sum) {
     const int r = e / DPAD, d = e - r * DPAD;
-    float v[4] = {o.x, o.y, o.z, o.w};
-    bool odd = false;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key's page is there, nothing is seen
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] *= inv;
-      odd |= !isfinite(v[j]);
-    }
+    const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     if (d < p.head_dim) {
       AT* to_at = reinterpret_cast<AT*>(p.out) + (int64_t(w.t) * p.n_heads + h0 + r) * p.head_dim + d;
       if (sizeof(AT) == 4) {
         *reinterpret_cast<float4*>(to_at) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
         AT h[4];
+        float none = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = DT<AT>::from_f32(v[j]);
+        for (int j = 0; j < 4; ++j) {
+          h[j] = DT<AT>::from_f32(v[j]);
+          none = fmaf(v[j], 0.f, none);
+        }
+        if (none != none && sum > 0.f) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (v[j] != v[j]) {
+              reinterpret_cast<uint16_t&>(h[j]) = kUnsettled;
+              any_unsettled = 1;
+            }
+        }
         *reinterpret_cast<uint2*>(to_at) = *reinterpret_cast<const uint2*>(h);
       }
     }
-    return Tile::kRedo && odd && d < p.head_dim;
-  };
-  // After the stores of a warp's 128 values from e0 on: the rows' blocks of 32 that have one that is not finite, again
-  auto store_again = [&](const Part& w, int h0, uint32_t odd, int e0) {
-    if (!odd) return;
-    __syncwarp();
-    for (int b = 0; b < 4; ++b)
-      if ((odd >> (8 * b)) & 0xff) row_again<AT>(p, w.k, w.k.hi - 1, w.t, h0 + (e0 + 32 * b) / DPAD, w.kvh, (e0 + 32 * b) % DPAD);
   };
   if (warp < WARPS) {
     int before = 0, small = 0;  // the share's tiles before this part; parts that were one warp's
@@ -928,10 +965,7 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       if (alone) {
         if (mine) {
           const bool odd = tile.finish(reinterpret_cast<AT*>(p.out) + (int64_t(part.t) * p.n_heads + h0) * p.head_dim, p.head_dim, rows);
-          if (Tile::kRedo && __any_sync(0xffffffffu, odd)) {
-            __syncwarp();
-            for (int i = 0; i < rows * DPAD; i += 32) row_again<AT>(p, part.k, part.k.hi - 1, part.t, h0 + i / DPAD, part.kvh, i % DPAD);
-          }
+          if (odd) any_unsettled = 1;
         }
         continue;
       }
@@ -957,10 +991,10 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
             o.x = fmaf(w.x, g, o.x); o.y = fmaf(w.y, g, o.y); o.z = fmaf(w.z, g, o.z); o.w = fmaf(w.w, g, o.w);
           }
         }
+        if (!here) continue;
         if (!part.left) {
-          const bool odd = here && store(part, h0, e, o, sum);
-          store_again(part, h0, __ballot_sync(0xffffffffu, odd), e0);
-        } else if (here) {
+          store(part, h0, e, o, sum);
+        } else {
           if (d == 0) { __stcg(slot + kSlotMax<Tile> + r, top); __stcg(slot + kSlotSum<Tile> + r, sum); }
           __stcg(reinterpret_cast<float4*>(slot + e), o);
         }
@@ -991,6 +1025,8 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
     is_last[threadIdx.x] = arrive(p.arrivals + slot_of(g.head, g.group * kGroup), g.members);
   }
   __syncthreads();
+  if ((is_last[0] | is_last[1] | any_unsettled) == 0) return;
+  unsigned joined = 0;
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
     if (!is_last[i]) continue;
@@ -1005,10 +1041,10 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       join<Tile>(p.slots, g.head, level == 0 ? g.group * kGroup : 0, level == 0 ? 1 : kGroup, level == 0 ? g.members : g.groups, rows, area,
                  [&](int e, float4 o, float top, float sum) {
                    const bool here = e < rows * DPAD;
+                   if (!here) return;
                    if (whole_part) {
-                     const bool odd = here && store(w, h0, e, o, sum);
-                     store_again(w, h0, __ballot_sync(0xffffffffu, odd), e - 4 * lane);
-                   } else if (here) {
+                     store(w, h0, e, o, sum);
+                   } else {
                      __stcg(reinterpret_cast<float4*>(to_slot + e), o);
                      if (e % DPAD == 0) { __stcg(to_slot + kSlotMax<Tile> + e / DPAD, top); __stcg(to_slot + kSlotSum<Tile> + e / DPAD, sum); }
                    }
@@ -1020,6 +1056,26 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
       if (!groups_done) break;
       whole_part = true;
     }
+    joined |= unsigned(whole_part) << i;
+  }
+
+  // Outputs that are not settled, now that the ring is empty: while one warp walked a sequence the others' waits would run out
+  if constexpr (Tile::kLookAgain) {
+    __syncthreads();
+    if (!any_unsettled) return;
+    auto again = [&](int t, int kvh, int tile, const Token& k) {
+      look_again<AT, DPAD, kThreads>(p, k, t, kvh, kvh * p.rep + tile * Tile::ROWS, min(Tile::ROWS, p.rep - tile * Tile::ROWS), reinterpret_cast<uint32_t*>(area));
+    };
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i)
+      if ((joined >> i) & 1) again(cut[i].t, cut[i].kvh, cut[i].tile, cut[i].k);
+    c.t = first.t; c.kvh = first.kvh; c.tile = first.tile; c.n = first.n; c.k = first.k;
+    c.seg = c.kvh * p.row_tiles + c.tile;
+    tile0 = first.tile0;
+    clip();
+    do {
+      if (c.u == 0 && stop == c.n) again(c.t, c.kvh, c.tile, c.k);
+    } while (advance());
   }
 }
 
