@@ -22,7 +22,7 @@ def reference(c, q, lengths, scale, softcap=0.0):
         page, slot = c.rows(i, n)
         k, v = (x[page, :, slot].double().repeat_interleave(h // c.kv_heads, 1) for x in (c.k, c.v))
         x = torch.einsum("hd,jhd->hj", q[i].double(), k) * scale
-        mag = torch.einsum("hd,jhd->hj", q[i].double().abs(), k.abs()).amax(1, keepdim=True) * abs(scale)
+        mag = torch.einsum("hd,jhd->hj", q[i].double().abs(), k.abs().nan_to_num(0, 0, 0)).amax(1, keepdim=True) * abs(scale)  # of finite scores
         dx = (d / 32 + 8 if q.dtype == torch.float32 else d / 16 * 4) * 2.0 ** -24 * mag
         if softcap:
             x = softcap * torch.tanh(x / softcap)
@@ -48,3 +48,57 @@ def test_caps_of_any_size(backend, dtype, heads, kv_heads, dim, page, softcap):
     got = run_attention(backend, c, q, pos, None, scale, softcap=softcap)
     ref, slack = reference(c, q, lengths, scale, softcap)
     assert_close(got, ref, slack, dtype)
+
+
+def finite_or_nan(got, ref, slack, dtype):
+    assert torch.equal(got.isnan(), ref.isnan()), f"NaN in {int(got.isnan().sum())} places for {int(ref.isnan().sum())}"
+    fine = ref.isfinite()
+    assert_close(got[fine], ref[fine], slack[fine], dtype)
+
+
+LENGTHS = [1, 17, 33, 65, 16, 49, 300, 2001, 1, 4000]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 128, 16), (24, 1, 64, 5), (6, 2, 256, 16)])
+@pytest.mark.parametrize("what", ["query", "newest key", "first key", "every seventh key", "infinite key", "plus infinity", "one key"])
+def test_scores_that_are_no_numbers(backend, dtype, heads, kv_heads, dim, page, what):
+    """NaN where a visible score is NaN, +infinity, or all of them are -infinity, wherever the key lies among the tiles, warps and CTAs; the other rows as ever."""
+    gen = torch.Generator(device="cuda").manual_seed(heads + len(what))
+    c = Cache(backend, gen, LENGTHS, kv_heads, dim, page, dtype)
+    q = normal(gen, (len(LENGTHS), heads, dim), dtype)
+    q[:, 0, 0] = q[:, 0, 0].abs() + 0.5
+    q[:, -1, 0] = -q[:, -1, 0].abs() - 0.5
+    inf, nan = float("inf"), float("nan")
+    for i, n in enumerate(LENGTHS):
+        c.fill(gen, i, n, dtype)
+        rows, slots = c.rows(i, n)
+        if what == "query" and i != 4:
+            q[i, i % heads, 3] = nan
+        elif what == "newest key":
+            c.k[rows[-1], i % kv_heads, slots[-1], 5] = nan
+        elif what == "first key":
+            c.k[rows[0], 0, slots[0], 5] = nan
+        elif what == "every seventh key" and i % 2:
+            c.k[rows[3::7], 0, slots[3::7], 0] = nan
+        elif what == "infinite key":  # the first head of the KV head 0 sees -infinity everywhere, others +infinity
+            c.k[rows, 0, slots, 0] = -inf
+        elif what == "plus infinity":
+            c.k[rows[n // 2], kv_heads - 1, slots[n // 2], 0] = inf
+        elif what == "one key":  # -infinity for the first head, all other scores finite
+            c.k[rows[n // 3], 0, slots[n // 3], 0] = -inf
+    pos = torch.tensor(LENGTHS, dtype=torch.int32, device="cuda") - 1
+    got = run_attention(backend, c, q, pos, None, dim ** -0.5)
+    finite_or_nan(got, *reference(c, q, LENGTHS, dim ** -0.5), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_a_row_that_sees_nothing_is_zeros_beside_nan(backend, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    c = Cache(backend, gen, [40, 40], 1, 64, 16, dtype)
+    for i in range(2):
+        c.fill(gen, i, 40, dtype)
+    q = normal(gen, (2, 2, 64), dtype)
+    q[:, 0, 0] = float("nan")
+    got = run_attention(backend, c, q, torch.tensor([39, -1], dtype=torch.int32, device="cuda"), None, 0.125)
+    assert got[0, 0].isnan().all() and got[0, 1].isfinite().all() and (got[1] == 0).all()

@@ -225,7 +225,9 @@ __device__ __noinline__ void look_again(const PagedArgs& p, const Token& k, int 
 template <typename AT> constexpr float kProbBias = 0.f;
 template <> constexpr float kProbBias<__half> = 10.f;
 
-// What a warp holds of the softmax of its keys, and how it takes a tile of them in: 16-bit types on the tensor cores.
+// What a warp holds of the softmax of its keys, and how it takes a tile of them in: 16-bit types on the tensor cores.  A maximum of -infinity says that no key has
+// been seen, and only that: from the first one on it is no less than -FLT_MAX, so that scores that are NaN (which no maximum keeps) or all -infinity end as NaN in
+// the sum or as a sum of zero, whose outputs are NaN, and not as the zeros of a row that sees nothing.
 // NT = 1: up to 8 query heads of a KV head, NT = 2: up to 16.
 template <typename AT_, int DPAD_, int NT>
 struct MmaTile {
@@ -316,7 +318,7 @@ struct MmaTile {
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-        nm[e] = fmaxf(m[nt][e], v);
+        nm[e] = fmaxf(fmaxf(m[nt][e], v), -FLT_MAX);
       }
       if (__any_sync(0xffffffffu, nm[0] != m[nt][0] || nm[1] != m[nt][1])) {
         float f[2];
@@ -334,8 +336,7 @@ struct MmaTile {
       float pr[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float mm = m[nt][e & 1];
-        pr[e] = mm == -INFINITY ? 0.f : exp2f(s[nt][e] - mm + kProbBias<AT>);
+        pr[e] = exp2f(s[nt][e] - m[nt][e & 1] + kProbBias<AT>);
         l[nt][e & 1] += pr[e];
       }
       uint32_t a[TERMS], b[TERMS];
@@ -393,7 +394,7 @@ struct MmaTile {
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        const float inv = v == 0.f ? 0.f : 1.f / v;
+        const float inv = m[nt][e] == -INFINITY ? 0.f : 1.f / v;
         const int r = nt * 8 + 2 * c + e;
         if (r < rows) {
           float none = 0.f;  // NaN if one of them is not finite
@@ -516,7 +517,7 @@ struct F32Tile {
       float top = x;  // over the keys of a row: lanes that differ in the key's bits
 #pragma unroll
       for (int b = 1 << (5 - kLog); b < KEYS << (5 - kLog); b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-      const float nm = fmaxf(m[s], top);
+      const float nm = fmaxf(fmaxf(m[s], top), -FLT_MAX);
       if (__any_sync(0xffffffffu, nm != m[s])) {
         const float f = nm == m[s] ? 1.f : exp2f(m[s] - nm);
         m[s] = nm;
@@ -528,7 +529,7 @@ struct F32Tile {
           for (int e = 0; e < E; ++e) o[s * kRowsOfSet + i][e] *= g;
         }
       }
-      pr[s] = nm == -INFINITY ? 0.f : exp2f(x - nm);
+      pr[s] = exp2f(x - nm);
       l[s] += pr[s];
     }
 #pragma unroll
@@ -566,7 +567,7 @@ struct F32Tile {
       float v = l[s];
 #pragma unroll
       for (int b = 1 << (5 - kLog); b < KEYS << (5 - kLog); b <<= 1) v += __shfl_xor_sync(0xffffffffu, v, b);
-      const float inv = v == 0.f ? 0.f : 1.f / v;
+      const float inv = m[s] == -INFINITY ? 0.f : 1.f / v;
 #pragma unroll
       for (int i = 0; i < kRowsOfSet; ++i) {
         const float f = __shfl_sync(0xffffffffu, inv, (i * KEYS) << (5 - kLog));
@@ -887,9 +888,9 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
   constexpr int kSmall = 4;
   float* area = reinterpret_cast<float*>(sm + p.stages * kStageBytes<Tile>);
   // Four neighbouring values of a row by each thread
-  auto store = [&](const Part& w, int h0, int e, float4 o, float sum) {
+  auto store = [&](const Part& w, int h0, int e, float4 o, float top, float sum) {
     const int r = e / DPAD, d = e - r * DPAD;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key's page is there, nothing is seen
+    const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // 0: no key's page is there, nothing is seen
     const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     if (d < p.head_dim) {
       AT* to_at = reinterpret_cast<AT*>(p.out) + (int64_t(w.t) * p.n_heads + h0 + r) * p.head_dim + d;
@@ -993,7 +994,7 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
         }
         if (!here) continue;
         if (!part.left) {
-          store(part, h0, e, o, sum);
+          store(part, h0, e, o, top, sum);
         } else {
           if (d == 0) { __stcg(slot + kSlotMax<Tile> + r, top); __stcg(slot + kSlotSum<Tile> + r, sum); }
           __stcg(reinterpret_cast<float4*>(slot + e), o);
@@ -1043,7 +1044,7 @@ __global__ void __launch_bounds__(32 + kConsumers<Tile>, Tile::CTAS)
                    const bool here = e < rows * DPAD;
                    if (!here) return;
                    if (whole_part) {
-                     store(w, h0, e, o, sum);
+                     store(w, h0, e, o, top, sum);
                    } else {
                      __stcg(reinterpret_cast<float4*>(to_slot + e), o);
                      if (e % DPAD == 0) { __stcg(to_slot + kSlotMax<Tile> + e / DPAD, top); __stcg(to_slot + kSlotSum<Tile> + e / DPAD, sum); }
