@@ -103,6 +103,10 @@ struct DecodeArgs {
   int32_t causal;
 };
 
+// The running maximum before the first key.  Not -infinity: scores that are NaN, which no maximum keeps, would leave it there, and what has -infinity for a maximum
+// could not be told from what has seen no key.
+constexpr float kNoMax = -FLT_MAX;
+
 // Partials of this CTA's warps -> the cluster's result.  sm: [warps][R] maxima, [warps][R] sums, [warps][R][D]
 // outputs, then the CTA's own merged [R], [R], [R][D].
 template <typename AT, int D, int R, int WARPS>
@@ -123,7 +127,7 @@ __device__ __forceinline__ void decode_merge(const DecodeArgs& p, float* sm, int
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float mw = wm[w * R + r];
-      const float f = mw == -INFINITY ? 0.f : exp2f((mw - m) * kLog2e);
+      const float f = exp2f((mw - m) * kLog2e);
       l = fmaf(wl[w * R + r], f, l);
       o = fmaf(wo[(w * R + r) * D + d], f, o);
     }
@@ -145,7 +149,7 @@ __device__ __forceinline__ void decode_merge(const DecodeArgs& p, float* sm, int
       const float* rl = p.splits > 1 ? cluster.map_shared_rank(cl, s) : cl;
       const float* ro = p.splits > 1 ? cluster.map_shared_rank(co, s) : co;
       const float ms = rm[r];
-      const float f = ms == -INFINITY ? 0.f : exp2f((ms - m) * kLog2e);
+      const float f = exp2f((ms - m) * kLog2e);
       l = fmaf(rl[r], f, l);
       o = fmaf(ro[r * D + d], f, o);
     }
@@ -235,7 +239,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attn_decode_mma_kernel(D
     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[nt][j][e] = 0.f;
-    m[nt][0] = m[nt][1] = -INFINITY;
+    m[nt][0] = m[nt][1] = kNoMax;
     l[nt][0] = l[nt][1] = 0.f;
   }
 
@@ -285,7 +289,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attn_decode_mma_kernel(D
         float f[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          f[c] = nm[c] == m[nt][c] ? 1.f : exp2f((m[nt][c] - nm[c]) * kLog2e);  // first keys: exp2(-inf) = 0 on zeros
+          f[c] = nm[c] == m[nt][c] ? 1.f : exp2f((m[nt][c] - nm[c]) * kLog2e);  // first keys: exp2(-huge) = 0 on zeros
           l[nt][c] *= f[c];
           m[nt][c] = nm[c];
         }
@@ -297,8 +301,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attn_decode_mma_kernel(D
       float pr[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float mm = m[nt][e & 1];
-        pr[e] = mm == -INFINITY ? 0.f : exp2f(fmaf(s[nt][e] - mm, kLog2e, kProbBias<AT>));  // no key visible yet: nothing to add
+        pr[e] = exp2f(fmaf(s[nt][e] - m[nt][e & 1], kLog2e, kProbBias<AT>));
         l[nt][e & 1] += pr[e];
       }
       uint32_t a[TERMS], c[TERMS];
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(128) attn_decode_f32_kernel(DecodeArgs p) {
     load_vec<V>(qp, q[r]);
 #pragma unroll
     for (int i = 0; i < V; ++i) o[r][i] = 0.f;
-    m[r] = -INFINITY;
+    m[r] = kNoMax;
     l[r] = 0.f;
     bound[r] = p.causal ? p.kv_len - p.q_len + qi + 1 : p.kv_len;
     mrow[r] = p.mask ? p.mask + int64_t(qi) * p.kv_len : nullptr;
@@ -406,19 +409,17 @@ __global__ void __launch_bounds__(128) attn_decode_f32_kernel(DecodeArgs p) {
         s[j] = key < bound[r] ? x : -INFINITY;
         nm = fmaxf(nm, s[j]);
       }
-      if (nm != -INFINITY) {
-        const float f = exp2f((m[r] - nm) * kLog2e);
-        m[r] = nm;
-        l[r] *= f;
+      const float f = exp2f((m[r] - nm) * kLog2e);
+      m[r] = nm;
+      l[r] *= f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[r][i] *= f;
+      for (int i = 0; i < V; ++i) o[r][i] *= f;
 #pragma unroll
-        for (int j = 0; j < KEYS; ++j) {
-          const float e = exp2f((s[j] - nm) * kLog2e);
-          l[r] += e;
+      for (int j = 0; j < KEYS; ++j) {
+        const float e = exp2f((s[j] - nm) * kLog2e);
+        l[r] += e;
 #pragma unroll
-          for (int i = 0; i < V; ++i) o[r][i] = fmaf(e, vf[j][i], o[r][i]);
-        }
+        for (int i = 0; i < V; ++i) o[r][i] = fmaf(e, vf[j][i], o[r][i]);
       }
     }
   }
