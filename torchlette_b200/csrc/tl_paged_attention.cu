@@ -1144,15 +1144,13 @@ int32_t secure_scratch(tl_ctx* ctx) {
   if (ctx->capturing || capture != cudaStreamCaptureStatusNone)
     return tl_set_error(ctx, TL_ERR_UNSUPPORTED, "tl_paged_attention: its scratch is not there yet during graph capture; run the call once before capturing");
   const size_t ctas = size_t(ctx->sm_count) * 2, bytes = ctas * (2 * kSlotFloats * sizeof(float) + 3 * sizeof(unsigned));
-  void* at = nullptr;
-  const cudaError_t e = ctx->pool.device_malloc(&at, bytes);
-  if (e != cudaSuccess) {
+  const cudaError_t e = tl_zeroed(ctx->pool, &ctx->paged_scratch, bytes, ctx->stream);
+  if (e == cudaErrorMemoryAllocation) {
     cudaGetLastError();
     return tl_set_error(ctx, TL_ERR_OOM, "tl_paged_attention: scratch of %zu bytes failed: %s", bytes, cudaGetErrorString(e));
   }
-  ctx->paged_scratch = at;
+  TL_CUDA(ctx, e);
   ctx->paged_scratch_bytes = bytes;
-  TL_CUDA(ctx, cudaMemsetAsync(at, 0, bytes, ctx->stream));
   return TL_OK;
 }
 

@@ -49,3 +49,14 @@ struct TlBlockPool {
   void fenced();           // a fence has just passed: waiting blocks become ready
   void trim(size_t keep);  // gives ready blocks back until at most `keep` bytes of them are left, the largest first
 };
+
+// Memory for the library itself that its kernels find zeroed: *out is set once the zeros are on the stream, and is what it was where one of the calls fails.
+inline cudaError_t tl_zeroed(TlBlockPool& pool, void** out, size_t bytes, cudaStream_t stream) {
+  void* at = nullptr;
+  cudaError_t e = pool.device_malloc(&at, bytes);
+  if (e != cudaSuccess) return e;
+  e = cudaMemsetAsync(at, 0, bytes, stream);
+  if (e == cudaSuccess) *out = at;
+  else cudaFree(at);
+  return e;
+}
