@@ -1,7 +1,9 @@
-"""Scratch whose zeroing fails is not kept: the next call would take its arrivals for zero.  tl_zeroed on a fake device, and that attention's scratch comes from it."""
+"""Scratch whose zeroing fails is not kept: the next call would take its arrivals for zero.  tl_zeroed on a fake device, and that the scratch with arrivals in it comes from there."""
 import os
 import re
 import subprocess
+
+import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "torchlette_b200", "csrc")
@@ -15,6 +17,7 @@ def test_zeroed_scratch(tmp_path):
     subprocess.run([exe], check=True)
 
 
-def test_attention_keeps_only_zeroed_scratch():
-    text = open(os.path.join(CSRC, "tl_paged_attention.cu")).read()
-    assert re.findall(r"tl_zeroed\(ctx->pool, &ctx->paged_scratch\b", text) and not re.search(r"paged_scratch = |device_malloc\(&ctx->paged_scratch", text)
+@pytest.mark.parametrize("source,name", [("tl_paged_attention.cu", "paged_scratch"), ("tl_api.cu", "zscratch"), ("tl_qgemv_stream.cu", "stream_scratch")])
+def test_only_zeroed_scratch_is_kept(source, name):
+    text = open(os.path.join(CSRC, source)).read()
+    assert f"tl_zeroed(ctx->pool, &ctx->{name}," in text and not re.search(rf"\b{name} = (?!nullptr)|device_malloc\(&ctx->{name}\b", text)

@@ -59,14 +59,14 @@ int32_t tl_ensure_zeroed_scratch(tl_ctx* ctx, size_t bytes, void** out) {
       ctx->zscratch_bytes = 0;
     }
     size_t want = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
-    cudaError_t e = ctx->pool.device_malloc(&ctx->zscratch, want);
-    if (e != cudaSuccess) {
+    const cudaError_t e = tl_zeroed(ctx->pool, &ctx->zscratch, want, ctx->stream);
+    if (e == cudaErrorMemoryAllocation) {
       cudaGetLastError();
       return tl_set_error(ctx, TL_ERR_OOM, "scratch allocation of %zu bytes failed: %s", want,
                           cudaGetErrorString(e));
     }
+    TL_CUDA(ctx, e);
     ctx->zscratch_bytes = want;
-    TL_CUDA(ctx, cudaMemsetAsync(ctx->zscratch, 0, want, ctx->stream));
   }
   *out = ctx->zscratch;
   return TL_OK;
