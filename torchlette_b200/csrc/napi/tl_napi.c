@@ -582,29 +582,80 @@ static int read_paged(napi_env env, napi_value o, tl_paged_cache* p) {
   napi_get_named_property(env, o, "maxPages", &v); p->max_pages = i32(env, v);
   return 1;
 }
+/* Whether a buffer handle holds the bytes that the call reads or writes through it (an address says nothing of what lies behind it): q of one type beside a cache of
+ * another would be read and answered past its end.  Extents are doubles, so that no product of theirs overflows; what is not positive is the library's to refuse. */
+static int holds(napi_env env, napi_value v, double bytes, const char* what) {
+  void* p = NULL;
+  if (type_of(env, v) != napi_external) return 1;
+  napi_get_value_external(env, v, &p);
+  if (!p || !((DevBuf*)p)->ptr || bytes <= (double)((DevBuf*)p)->bytes) return 1;
+  char text[96] = "tlcuda: the call reaches past the end of ";
+  strncat(text, what, sizeof(text) - strlen(text) - 1);
+  napi_throw_error(env, NULL, text);
+  return 0;
+}
+static double elem_bytes(int32_t dtype) { return dtype == TL_F32 ? 4 : dtype == TL_F16 || dtype == TL_BF16 ? 2 : 0; }
+/* of [tokens, heads, dim] with these strides in elements */
+static double extent(int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim, int32_t dtype) {
+  return (((double)tokens - 1) * (double)token_stride + ((double)heads - 1) * (double)head_stride + (double)dim) * elem_bytes(dtype);
+}
+static int holds_paged(napi_env env, napi_value o, const tl_paged_cache* p, napi_value positions, napi_value token_seq, int64_t tokens) {
+  napi_value v;
+  const double pages = (double)p->n_pages * p->n_kv_heads * p->page_size * p->head_dim * elem_bytes(p->dtype);
+  napi_get_named_property(env, o, "kPages", &v);
+  if (!holds(env, v, pages, "kPages")) return 0;
+  napi_get_named_property(env, o, "vPages", &v);
+  if (!holds(env, v, pages, "vPages")) return 0;
+  napi_get_named_property(env, o, "pageTable", &v);
+  if (!holds(env, v, 4.0 * p->n_seqs * p->max_pages, "pageTable")) return 0;
+  return holds(env, positions, 4.0 * (double)tokens, "positions") && holds(env, token_seq, 4.0 * (double)tokens, "tokenSeq");
+}
 /* pagedAppend(ctx, cache, positions, tokenSeq | null, tokens, q | null, qTokenStride, qHeadStride, heads, qOut | null, outTokenStride, outHeadStride,
- * k, kTokenStride, kHeadStride, v, vTokenStride, vHeadStride, qWeight | null, kWeight | null, weightDtype, eps, cos | null, sin | null, tableRows) */
+ * k, kTokenStride, kHeadStride, v, vTokenStride, vHeadStride, qWeight | null, kWeight | null, weightDtype, eps, cos | null, sin | null, tableRows).
+ * Buffer handles hold the rows of all tokens, the ones that are not there included. */
 FN(PagedAppend) {
   ARGS(25); CTX(0); tl_paged_cache p;
   if (!read_paged(env, argv[1], &p)) return undef(env);
-  return check(env, c, tl_paged_append(c, &p, (const int32_t*)dptr(env, argv[2]), (const int32_t*)dptr(env, argv[3]), i64(env, argv[4]), dptr(env, argv[5]),
-                                       i64(env, argv[6]), i64(env, argv[7]), i64(env, argv[8]), dptr(env, argv[9]), i64(env, argv[10]), i64(env, argv[11]),
+  const int64_t tokens = i64(env, argv[4]), heads = i64(env, argv[8]), rows = i64(env, argv[24]);
+  const int32_t wd = i32(env, argv[20]);
+  if (tokens > 0 &&
+      (!holds_paged(env, argv[1], &p, argv[2], argv[3], tokens) ||
+       !holds(env, argv[5], extent(tokens, i64(env, argv[6]), heads, i64(env, argv[7]), p.head_dim, p.dtype), "q") ||
+       !holds(env, argv[9], extent(tokens, i64(env, argv[10]), heads, i64(env, argv[11]), p.head_dim, p.dtype), "qOut") ||
+       !holds(env, argv[12], extent(tokens, i64(env, argv[13]), p.n_kv_heads, i64(env, argv[14]), p.head_dim, p.dtype), "k") ||
+       !holds(env, argv[15], extent(tokens, i64(env, argv[16]), p.n_kv_heads, i64(env, argv[17]), p.head_dim, p.dtype), "v") ||
+       !holds(env, argv[18], p.head_dim * elem_bytes(wd), "qWeight") || !holds(env, argv[19], p.head_dim * elem_bytes(wd), "kWeight") ||
+       !holds(env, argv[22], 2.0 * (double)rows * p.head_dim, "cos") || !holds(env, argv[23], 2.0 * (double)rows * p.head_dim, "sin")))
+    return undef(env);
+  return check(env, c, tl_paged_append(c, &p, (const int32_t*)dptr(env, argv[2]), (const int32_t*)dptr(env, argv[3]), tokens, dptr(env, argv[5]),
+                                       i64(env, argv[6]), i64(env, argv[7]), heads, dptr(env, argv[9]), i64(env, argv[10]), i64(env, argv[11]),
                                        dptr(env, argv[12]), i64(env, argv[13]), i64(env, argv[14]), dptr(env, argv[15]), i64(env, argv[16]), i64(env, argv[17]),
-                                       dptr(env, argv[18]), dptr(env, argv[19]), i32(env, argv[20]), (float)f64(env, argv[21]),
-                                       (const float*)dptr(env, argv[22]), (const float*)dptr(env, argv[23]), i64(env, argv[24])));
+                                       dptr(env, argv[18]), dptr(env, argv[19]), wd, (float)f64(env, argv[21]),
+                                       (const float*)dptr(env, argv[22]), (const float*)dptr(env, argv[23]), rows));
 }
 /* pagedAttention(ctx, cache, positions, tokenSeq | null, tokens, q, qTokenStride, qHeadStride, heads, out, scale, softcap, window, slopes | null) */
 FN(PagedAttention) {
   ARGS(14); CTX(0); tl_paged_cache p;
   if (!read_paged(env, argv[1], &p)) return undef(env);
-  return check(env, c, tl_paged_attention(c, &p, (const int32_t*)dptr(env, argv[2]), (const int32_t*)dptr(env, argv[3]), i64(env, argv[4]), dptr(env, argv[5]),
-                                          i64(env, argv[6]), i64(env, argv[7]), i64(env, argv[8]), dptr(env, argv[9]), (float)f64(env, argv[10]),
+  const int64_t tokens = i64(env, argv[4]), heads = i64(env, argv[8]);
+  if (tokens > 0 && (!holds_paged(env, argv[1], &p, argv[2], argv[3], tokens) ||
+                     !holds(env, argv[5], extent(tokens, i64(env, argv[6]), heads, i64(env, argv[7]), p.head_dim, p.dtype), "q") ||
+                     !holds(env, argv[9], (double)tokens * (double)heads * p.head_dim * elem_bytes(p.dtype), "out") ||
+                     !holds(env, argv[13], 4.0 * (double)heads, "slopes")))
+    return undef(env);
+  return check(env, c, tl_paged_attention(c, &p, (const int32_t*)dptr(env, argv[2]), (const int32_t*)dptr(env, argv[3]), tokens, dptr(env, argv[5]),
+                                          i64(env, argv[6]), i64(env, argv[7]), heads, dptr(env, argv[9]), (float)f64(env, argv[10]),
                                           (float)f64(env, argv[11]), i32(env, argv[12]), (const float*)dptr(env, argv[13])));
 }
 /* sample(ctx, logits, dtype, rows, vocab, rowStride, temperature | null, topK | null, topP | null, minP | null, uniforms | null, out) */
 FN(Sample) {
   ARGS(12); CTX(0);
-  return check(env, c, tl_sample(c, dptr(env, argv[1]), i32(env, argv[2]), i64(env, argv[3]), i64(env, argv[4]), i64(env, argv[5]),
+  const int64_t rows = i64(env, argv[3]), vocab = i64(env, argv[4]);
+  static const char* const kNames[] = {"temperature", "topK", "topP", "minP", "uniforms", "out"};
+  if (rows > 0 && !holds(env, argv[1], (((double)rows - 1) * (double)i64(env, argv[5]) + (double)vocab) * elem_bytes(i32(env, argv[2])), "logits")) return undef(env);
+  for (int i = 0; i < 6; ++i)
+    if (!holds(env, argv[6 + i], 4.0 * (double)rows, kNames[i])) return undef(env);
+  return check(env, c, tl_sample(c, dptr(env, argv[1]), i32(env, argv[2]), rows, vocab, i64(env, argv[5]),
                                  (const float*)dptr(env, argv[6]), (const int32_t*)dptr(env, argv[7]), (const float*)dptr(env, argv[8]),
                                  (const float*)dptr(env, argv[9]), (const float*)dptr(env, argv[10]), (int32_t*)dptr(env, argv[11])));
 }

@@ -214,40 +214,72 @@ export function attention(q: CudaTensor, kCache: CudaTensor, vCache: CudaTensor,
 /** kPages, vPages [nPages, kvH, pageSize, D] and pageTable i32 [nSeqs, maxPages]; position p of a sequence lies in page
  * pageTable[seq][p / pageSize] at p % pageSize.  A contiguous cache [B, kvH, capacity, D] has pageSize == capacity and a table [[0], [1], ...]. */
 export interface PagedCache { kPages: CudaTensor; vPages: CudaTensor; pageTable: CudaTensor }
-const pagedArg = (c: PagedCache): any => ({
-  kPages: c.kPages.buffer, vPages: c.vPages.buffer, pageTable: c.pageTable.buffer, nPages: c.kPages.shape[0], kvHeads: c.kPages.shape[1],
-  pageSize: c.kPages.shape[2], headDim: c.kPages.shape[3], dtype: DTYPE_ID[c.kPages.dtype as string], nSeqs: c.pageTable.shape[0],
-  maxPages: c.pageTable.shape[1],
-});
+function refuseUnless(ok: boolean, message: string): void {
+  if (!ok) throw new Error(message);
+}
+/** Contiguous, of the dtype and of one of the shapes; an absent tensor fits. */
+const fits = (t: CudaTensor | null | undefined, dtype: string, ...shapes: number[][]): boolean =>
+  !t || (!t.transposed && t.dtype === dtype && shapes.some((s) => s.length === t.shape.length && s.every((n, i) => n === t.shape[i])));
+const at = (t?: CudaTensor | null): any => (t ? t.buffer : null);
+/** The cache that pagedAppend fills and pagedAttention reads, over pages and a table that the caller owns. */
+export function createPagedCache(kPages: CudaTensor, vPages: CudaTensor, pageTable: CudaTensor): PagedCache {
+  const cache = { kPages, vPages, pageTable };
+  pagedArg(cache);
+  return cache;
+}
+function pagedArg(c: PagedCache): any {
+  const dtype = c.kPages.dtype as string, shape = c.kPages.shape;
+  refuseUnless(dtype in DTYPE_ID && shape.length === 4 && shape.every((n, i) => i === 0 || n > 0) && fits(c.kPages, dtype, shape) && fits(c.vPages, dtype, shape),
+               "paged cache: kPages and vPages are [nPages, kvH, pageSize, D] of one dtype");
+  refuseUnless(c.pageTable.shape.length === 2 && fits(c.pageTable, "i32", c.pageTable.shape), "paged cache: pageTable is i32 [nSeqs, maxPages]");
+  return { kPages: c.kPages.buffer, vPages: c.vPages.buffer, pageTable: c.pageTable.buffer, nPages: shape[0], kvHeads: shape[1], pageSize: shape[2], headDim: shape[3],
+           dtype: DTYPE_ID[dtype], nSeqs: c.pageTable.shape[0], maxPages: c.pageTable.shape[1] };
+}
+function tokensOf(who: string, positions: CudaTensor, tokenSeq?: CudaTensor): number {
+  refuseUnless(positions.shape.length === 1 && fits(positions, "i32", positions.shape), `${who}: positions are i32 [tokens]`);
+  refuseUnless(fits(tokenSeq, "i32", positions.shape), `${who}: tokenSeq is i32 [tokens]`);
+  return positions.shape[0];
+}
 /** The per-head norms of q and k, the rotation at each token's position and the append of k and v, one launch; the new q [T, H, D].
  * q [T, H, D], k and v [T, kvH, D]; positions i32 [T] (negative: not there), tokenSeq i32 [T] (absent: token t is of sequence t). */
 export function pagedAppend(cache: PagedCache, positions: CudaTensor, q: CudaTensor, k: CudaTensor, v: CudaTensor,
                             config: { cos?: CudaTensor; sin?: CudaTensor; qNorm?: CudaTensor; kNorm?: CudaTensor; eps?: number;
                                       tokenSeq?: CudaTensor } = {}): CudaTensor {
-  const p = pagedArg(cache), d = p.headDim, g = p.kvHeads, tokens = positions.shape[0], heads = numel(q.shape) / (tokens * d);
-  const out = empty([tokens, heads, d], q.dtype as string), norm = config.qNorm ?? config.kNorm;
-  const at = (t?: CudaTensor): any => (t ? t.buffer : null);
-  addon.pagedAppend(need(), p, positions.buffer, at(config.tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, heads * d, d, k.buffer, g * d, d,
-                    v.buffer, g * d, d, at(config.qNorm), at(config.kNorm), norm ? DTYPE_ID[norm.dtype as string] : 0, config.eps ?? 1e-6,
-                    at(config.cos), at(config.sin), config.cos ? config.cos.shape[0] : 0);
+  const { cos, sin, qNorm, kNorm, tokenSeq } = config, p = pagedArg(cache), d = p.headDim, g = p.kvHeads, dtype = cache.kPages.dtype as string;
+  const tokens = tokensOf("pagedAppend", positions, tokenSeq), norm = qNorm ?? kNorm, heads = q.shape.length === 3 ? q.shape[1] : q.shape[1] / d;
+  refuseUnless(heads >= 1 && Number.isInteger(heads) && fits(q, dtype, [tokens, heads, d], [tokens, heads * d]), "pagedAppend: q is [tokens, H, D] of the cache's dtype");
+  refuseUnless(fits(k, dtype, [tokens, g, d], [tokens, g * d]) && fits(v, dtype, [tokens, g, d], [tokens, g * d]), "pagedAppend: k and v are [tokens, kvH, D] of the cache's dtype");
+  refuseUnless(!norm || (fits(qNorm, norm.dtype as string, [d]) && fits(kNorm, norm.dtype as string, [d]) && (norm.dtype as string) in DTYPE_ID),
+               "pagedAppend: qNorm and kNorm are [D] of one dtype");
+  const rows = cos ? cos.shape[0] : 0;
+  refuseUnless(!cos === !sin && fits(cos, "f32", [rows, d / 2]) && fits(sin, "f32", [rows, d / 2]), "pagedAppend: cos and sin are f32 [rows, D/2]");
+  const out = empty([tokens, heads, d], dtype);
+  addon.pagedAppend(need(), p, positions.buffer, at(tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, heads * d, d, k.buffer, g * d, d, v.buffer, g * d, d,
+                    at(qNorm), at(kNorm), norm ? DTYPE_ID[norm.dtype as string] : 0, config.eps ?? 1e-6, at(cos), at(sin), rows);
   return out;
 }
-/** Attention of each token over its own sequence's positions up to its own: q [T, H, D] -> [T, H * D]. */
+/** Attention of each token over its own sequence's positions up to its own: q [T, H, D] or [T, H * D] -> [T, H * D]. */
 export function pagedAttention(cache: PagedCache, positions: CudaTensor, q: CudaTensor, scale: number,
                                config: { softcap?: number; window?: number; slopes?: CudaTensor; tokenSeq?: CudaTensor } = {}): CudaTensor {
-  const p = pagedArg(cache), d = p.headDim, tokens = positions.shape[0], heads = numel(q.shape) / (tokens * d);
-  const out = empty([tokens, heads * d], q.dtype as string);
-  addon.pagedAttention(need(), p, positions.buffer, config.tokenSeq ? config.tokenSeq.buffer : null, tokens, q.buffer, heads * d, d, heads, out.buffer,
-                       scale, config.softcap ?? 0, config.window ?? 0, config.slopes ? config.slopes.buffer : null);
+  const { slopes, tokenSeq } = config, p = pagedArg(cache), d = p.headDim, dtype = cache.kPages.dtype as string;
+  const tokens = tokensOf("pagedAttention", positions, tokenSeq), heads = q.shape.length === 3 ? q.shape[1] : q.shape.length === 2 ? q.shape[1] / d : 0;
+  refuseUnless(heads >= 1 && Number.isInteger(heads) && fits(q, dtype, [tokens, heads, d], [tokens, heads * d]), "pagedAttention: q is [tokens, H, D] of the cache's dtype");
+  refuseUnless(fits(slopes, "f32", [heads]), "pagedAttention: slopes are f32 [H]");
+  const out = empty([tokens, heads * d], dtype);
+  addon.pagedAttention(need(), p, positions.buffer, at(tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, scale, config.softcap ?? 0, config.window ?? 0, at(slopes));
   return out;
 }
-/** A token of each row of logits [rows, vocab] from uniforms f32 [rows]; parameters f32 (topK: i32) [rows] or absent.  Returns i32 [rows]. */
+/** A token of each row of logits [rows, vocab] (any leading dims) from uniforms f32 [rows]; parameters f32 (topK: i32) [rows] or absent.  Returns i32 [rows]. */
 export function sample(logits: CudaTensor, uniforms: CudaTensor | null,
                        config: { temperature?: CudaTensor; topK?: CudaTensor; topP?: CudaTensor; minP?: CudaTensor } = {}): CudaTensor {
-  const vocab = logits.shape[logits.shape.length - 1], rows = numel(logits.shape) / vocab, out = empty([rows], "i32");
-  const at = (t?: CudaTensor | null): any => (t ? t.buffer : null);
-  addon.sample(need(), logits.buffer, DTYPE_ID[logits.dtype as string], rows, vocab, vocab, at(config.temperature), at(config.topK), at(config.topP),
-               at(config.minP), at(uniforms), out.buffer);
+  const { temperature, topK, topP, minP } = config, dtype = logits.dtype as string;
+  const vocab = logits.shape[logits.shape.length - 1], rows = numel(logits.shape.slice(0, -1));
+  refuseUnless(logits.shape.length >= 1 && dtype in DTYPE_ID && fits(logits, dtype, logits.shape), "sample: logits are [rows, vocab] of f32, f16 or bf16");
+  refuseUnless(fits(uniforms, "f32", [rows]) && fits(temperature, "f32", [rows]) && fits(topP, "f32", [rows]) && fits(minP, "f32", [rows]),
+               "sample: uniforms, temperature, topP and minP are f32 [rows]");
+  refuseUnless(fits(topK, "i32", [rows]), "sample: topK is i32 [rows]");
+  const out = empty([rows], "i32");
+  addon.sample(need(), logits.buffer, DTYPE_ID[dtype], rows, vocab, vocab, at(temperature), at(topK), at(topP), at(minP), at(uniforms), out.buffer);
   return out;
 }
 
