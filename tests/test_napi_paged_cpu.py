@@ -26,9 +26,9 @@ def _function(name):
     return text[at:text.index("\n}\n", at)]
 
 
-@pytest.mark.parametrize("name,tensors", [("pagedAppend", ["positions", "tokenSeq", "q", "k", "v", "qNorm", "kNorm", "cos", "sin"]),
-                                          ("pagedAttention", ["positions", "tokenSeq", "q", "slopes"]),
-                                          ("sample", ["logits", "uniforms", "temperature", "topK", "topP", "minP"])])
+@pytest.mark.parametrize("name,tensors", [("pagedAppend", ["positions", "tokenSeq", "q", "k", "v", "out", "qNorm", "kNorm", "cos", "sin"]),
+                                          ("pagedAttention", ["positions", "tokenSeq", "q", "out", "slopes"]),
+                                          ("sample", ["logits", "uniforms", "temperature", "topK", "topP", "minP", "out"])])
 def test_typescript_looks_at_every_tensor(name, tensors):
     """Each tensor whose buffer is handed over is named in a check before the addon is called; what is new has the cache's type, not q's."""
     body = _function(name)
@@ -37,3 +37,10 @@ def test_typescript_looks_at_every_tensor(name, tensors):
     for t in tensors:
         assert re.search(rf"\b{t}\b", checked), t
     assert "q.dtype" not in re.sub(r"(?:fits|refuseUnless)\([^;]*;", "", body)
+
+
+@pytest.mark.parametrize("name", ["pagedAppend", "pagedAttention", "sample"])
+def test_typescript_needs_no_allocation(name):
+    """A capture takes no allocations: each call writes where it is told to."""
+    body = _function(name)
+    assert "config.out ?? empty(" in body and body.count("empty(") == 1

@@ -240,45 +240,76 @@ function tokensOf(who: string, positions: CudaTensor, tokenSeq?: CudaTensor): nu
   refuseUnless(fits(tokenSeq, "i32", positions.shape), `${who}: tokenSeq is i32 [tokens]`);
   return positions.shape[0];
 }
-/** The per-head norms of q and k, the rotation at each token's position and the append of k and v, one launch; the new q [T, H, D].
- * q [T, H, D], k and v [T, kvH, D]; positions i32 [T] (negative: not there), tokenSeq i32 [T] (absent: token t is of sequence t). */
-export function pagedAppend(cache: PagedCache, positions: CudaTensor, q: CudaTensor, k: CudaTensor, v: CudaTensor,
-                            config: { cos?: CudaTensor; sin?: CudaTensor; qNorm?: CudaTensor; kNorm?: CudaTensor; eps?: number;
-                                      tokenSeq?: CudaTensor } = {}): CudaTensor {
-  const { cos, sin, qNorm, kNorm, tokenSeq } = config, p = pagedArg(cache), d = p.headDim, g = p.kvHeads, dtype = cache.kPages.dtype as string;
-  const tokens = tokensOf("pagedAppend", positions, tokenSeq), norm = qNorm ?? kNorm, heads = q.shape.length === 3 ? q.shape[1] : q.shape[1] / d;
-  refuseUnless(heads >= 1 && Number.isInteger(heads) && fits(q, dtype, [tokens, heads, d], [tokens, heads * d]), "pagedAppend: q is [tokens, H, D] of the cache's dtype");
-  refuseUnless(fits(k, dtype, [tokens, g, d], [tokens, g * d]) && fits(v, dtype, [tokens, g, d], [tokens, g * d]), "pagedAppend: k and v are [tokens, kvH, D] of the cache's dtype");
+export interface PagedAppendConfig {
+  cos?: CudaTensor; sin?: CudaTensor; qNorm?: CudaTensor; kNorm?: CudaTensor; eps?: number; tokenSeq?: CudaTensor; headsFirst?: boolean; out?: CudaTensor;
+}
+/** The per-head norms of q and k (qNorm, kNorm [D], where given), the rotation at each token's position (cos / sin f32 [rows, D/2], where given) and the append of k and v,
+ * one launch; the new q [T, H, D].  q is [T, H, D] or [T, H * D], k and v [T, kvH, D] or [T, kvH * D]; with headsFirst all of them, the result too, are
+ * [heads, T, D].  k = v = null: q holds the rows of one product, [T, (H + 2 kvH) * D].  q = null: k and v alone, and null is returned.  out: the result's place, q itself
+ * among them.  positions i32 [T] (negative: not there), tokenSeq i32 [T] (absent: token t is of sequence t). */
+export function pagedAppend(cache: PagedCache, positions: CudaTensor, q: CudaTensor, k: CudaTensor | null, v: CudaTensor | null, config?: PagedAppendConfig): CudaTensor;
+export function pagedAppend(cache: PagedCache, positions: CudaTensor, q: null, k: CudaTensor, v: CudaTensor, config?: PagedAppendConfig): null;
+export function pagedAppend(cache: PagedCache, positions: CudaTensor, q: CudaTensor | null, k: CudaTensor | null, v: CudaTensor | null,
+                            config: PagedAppendConfig = {}): CudaTensor | null {
+  const { cos, sin, qNorm, kNorm, tokenSeq, headsFirst = false } = config;
+  const p = pagedArg(cache), d = p.headDim, g = p.kvHeads, dtype = cache.kPages.dtype as string, esz = DTYPE_BYTES[dtype];
+  const tokens = tokensOf("pagedAppend", positions, tokenSeq), norm = qNorm ?? kNorm;
+  refuseUnless(!k === !v, "pagedAppend: k and v come together");
   refuseUnless(!norm || (fits(qNorm, norm.dtype as string, [d]) && fits(kNorm, norm.dtype as string, [d]) && (norm.dtype as string) in DTYPE_ID),
                "pagedAppend: qNorm and kNorm are [D] of one dtype");
   const rows = cos ? cos.shape[0] : 0;
   refuseUnless(!cos === !sin && fits(cos, "f32", [rows, d / 2]) && fits(sin, "f32", [rows, d / 2]), "pagedAppend: cos and sin are f32 [rows, D/2]");
-  const out = empty([tokens, heads, d], dtype);
-  addon.pagedAppend(need(), p, positions.buffer, at(tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, heads * d, d, k.buffer, g * d, d, v.buffer, g * d, d,
+  // [token, head] strides in elements
+  const strides = (heads: number): [number, number] => (headsFirst ? [d, tokens * d] : [heads * d, d]);
+  const shapes = (heads: number): number[][] => (headsFirst ? [[heads, tokens, d]] : [[tokens, heads, d], [tokens, heads * d]]);
+  let heads = 0, qs: [number, number] = [0, 0], ks = strides(g), kAt = at(k), vAt = at(v);
+  if (!k || !v) {
+    const width = q ? q.shape[1] : 0;
+    refuseUnless(!!q && !headsFirst && fits(q, dtype, [tokens, width]) && width % d === 0 && width > 2 * g * d, "pagedAppend: q alone is [tokens, (H + 2 kvH) * D] of the cache's dtype");
+    heads = width / d - 2 * g;
+    qs = ks = [width, d];
+    if (tokens > 0) {
+      kAt = addon.view(at(q), heads * d * esz);
+      vAt = addon.view(at(q), (heads + g) * d * esz);
+    }
+  } else {
+    refuseUnless(fits(k, dtype, ...shapes(g)) && fits(v, dtype, ...shapes(g)), "pagedAppend: k and v are [tokens, kvH, D] of the cache's dtype");
+    if (q) {
+      heads = headsFirst ? q.shape[0] : q.shape.length === 3 ? q.shape[1] : q.shape[1] / d;
+      refuseUnless(heads >= 1 && Number.isInteger(heads) && fits(q, dtype, ...shapes(heads)), "pagedAppend: q is [tokens, H, D] of the cache's dtype");
+      qs = strides(heads);
+    }
+  }
+  refuseUnless(!!q || !config.out, "pagedAppend: out is the new q's");
+  refuseUnless(fits(config.out, dtype, ...shapes(heads)), "pagedAppend: out is q's shape, of the cache's dtype");
+  const out = q ? config.out ?? empty(shapes(heads)[0], dtype) : null, os = strides(heads);
+  addon.pagedAppend(need(), p, positions.buffer, at(tokenSeq), tokens, at(q), qs[0], qs[1], heads, at(out), os[0], os[1], kAt, ks[0], ks[1], vAt, ks[0], ks[1],
                     at(qNorm), at(kNorm), norm ? DTYPE_ID[norm.dtype as string] : 0, config.eps ?? 1e-6, at(cos), at(sin), rows);
   return out;
 }
-/** Attention of each token over its own sequence's positions up to its own: q [T, H, D] or [T, H * D] -> [T, H * D]. */
+/** Attention of each token over its own sequence's positions up to its own: q [T, H, D] or [T, H * D] -> [T, H * D], in `out` where given. */
 export function pagedAttention(cache: PagedCache, positions: CudaTensor, q: CudaTensor, scale: number,
-                               config: { softcap?: number; window?: number; slopes?: CudaTensor; tokenSeq?: CudaTensor } = {}): CudaTensor {
+                               config: { softcap?: number; window?: number; slopes?: CudaTensor; tokenSeq?: CudaTensor; out?: CudaTensor } = {}): CudaTensor {
   const { slopes, tokenSeq } = config, p = pagedArg(cache), d = p.headDim, dtype = cache.kPages.dtype as string;
   const tokens = tokensOf("pagedAttention", positions, tokenSeq), heads = q.shape.length === 3 ? q.shape[1] : q.shape.length === 2 ? q.shape[1] / d : 0;
   refuseUnless(heads >= 1 && Number.isInteger(heads) && fits(q, dtype, [tokens, heads, d], [tokens, heads * d]), "pagedAttention: q is [tokens, H, D] of the cache's dtype");
   refuseUnless(fits(slopes, "f32", [heads]), "pagedAttention: slopes are f32 [H]");
-  const out = empty([tokens, heads * d], dtype);
+  refuseUnless(fits(config.out, dtype, [tokens, heads * d], [tokens, heads, d]), "pagedAttention: out is [tokens, H * D] of the cache's dtype");
+  const out = config.out ?? empty([tokens, heads * d], dtype);
   addon.pagedAttention(need(), p, positions.buffer, at(tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, scale, config.softcap ?? 0, config.window ?? 0, at(slopes));
   return out;
 }
-/** A token of each row of logits [rows, vocab] (any leading dims) from uniforms f32 [rows]; parameters f32 (topK: i32) [rows] or absent.  Returns i32 [rows]. */
+/** A token of each row of logits [rows, vocab] (any leading dims) from uniforms f32 [rows]; parameters f32 (topK: i32) [rows] or absent.  Returns i32 [rows], in `out`
+ * where given. */
 export function sample(logits: CudaTensor, uniforms: CudaTensor | null,
-                       config: { temperature?: CudaTensor; topK?: CudaTensor; topP?: CudaTensor; minP?: CudaTensor } = {}): CudaTensor {
+                       config: { temperature?: CudaTensor; topK?: CudaTensor; topP?: CudaTensor; minP?: CudaTensor; out?: CudaTensor } = {}): CudaTensor {
   const { temperature, topK, topP, minP } = config, dtype = logits.dtype as string;
   const vocab = logits.shape[logits.shape.length - 1], rows = numel(logits.shape.slice(0, -1));
   refuseUnless(logits.shape.length >= 1 && dtype in DTYPE_ID && fits(logits, dtype, logits.shape), "sample: logits are [rows, vocab] of f32, f16 or bf16");
   refuseUnless(fits(uniforms, "f32", [rows]) && fits(temperature, "f32", [rows]) && fits(topP, "f32", [rows]) && fits(minP, "f32", [rows]),
                "sample: uniforms, temperature, topP and minP are f32 [rows]");
-  refuseUnless(fits(topK, "i32", [rows]), "sample: topK is i32 [rows]");
-  const out = empty([rows], "i32");
+  refuseUnless(fits(topK, "i32", [rows]) && fits(config.out, "i32", [rows]), "sample: topK and out are i32 [rows]");
+  const out = config.out ?? empty([rows], "i32");
   addon.sample(need(), logits.buffer, DTYPE_ID[dtype], rows, vocab, vocab, at(temperature), at(topK), at(topP), at(minP), at(uniforms), out.buffer);
   return out;
 }
