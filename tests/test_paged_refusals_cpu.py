@@ -1,0 +1,15 @@
+"""More of what the backend refuses, or passes on as it is meant, in the paged cache's calls."""
+import pytest
+
+from test_paged_cpu import _paged, _t, be  # noqa: F401
+from torchlette_b200 import backend as tb
+
+
+def test_transposed_tables_are_refused(be):  # noqa: F811
+    cache, pos, q, k, v = _paged(be), _t(be, [3], "i32"), _t(be, [3, 4, 64]), _t(be, [3, 2, 64]), _t(be, [3, 2, 64])
+    good, turned = _t(be, [50, 32], "f32"), be.ops.transpose(_t(be, [32, 50], "f32"))
+    assert turned.shape == good.shape
+    for cos, sin in ((turned, good), (good, turned)):
+        with pytest.raises(tb.TlError, match="cos and sin"):
+            be.ops.pagedAppend(cache, pos, q, k, v, cos, sin)
+    assert not [c for c in be.calls if c[0] != "tl_alloc"]

@@ -397,7 +397,8 @@ class CudaOps:
             _refuse("pagedAppend: qNorm and kNorm are [D] of one dtype")
         if (cos is None) != (sin is None):
             _refuse("pagedAppend: cos and sin come together")
-        if cos is not None and (cos.dtype != "f32" or sin.dtype != "f32" or len(cos.shape) != 2 or cos.shape != sin.shape or 2 * cos.shape[1] != d):
+        if cos is not None and (cos.dtype != "f32" or sin.dtype != "f32" or len(cos.shape) != 2 or cos.shape != sin.shape or 2 * cos.shape[1] != d or
+                                cos.transposed or sin.transposed):
             _refuse("pagedAppend: cos and sin are f32 [rows, D/2]")
         if q_at is None:
             if out is not None:
