@@ -13,3 +13,10 @@ def test_transposed_tables_are_refused(be):  # noqa: F811
         with pytest.raises(tb.TlError, match="cos and sin"):
             be.ops.pagedAppend(cache, pos, q, k, v, cos, sin)
     assert not [c for c in be.calls if c[0] != "tl_alloc"]
+
+
+@pytest.mark.parametrize("shape", [[9, 0, 16, 64], [9, 2, 0, 64], [9, 2, 16, 0]])
+def test_a_cache_without_heads_slots_or_dimensions_is_refused(be, shape):  # noqa: F811
+    with pytest.raises(tb.TlError, match="createPagedCache"):
+        tb.PagedCache(be, _t(be, shape), _t(be, shape), _t(be, [3, 4], "i32"))
+    tb.PagedCache(be, _t(be, [0, 2, 16, 64]), _t(be, [0, 2, 16, 64]), _t(be, [0, 0], "i32"))  # one without pages yet is not

@@ -164,7 +164,7 @@ class PagedCache:
     pageSize == capacity and a table [[0], [1], ...]."""
 
     def __init__(self, backend, kPages: CudaTensor, vPages: CudaTensor, pageTable: CudaTensor):
-        if len(kPages.shape) != 4 or kPages.shape != vPages.shape or kPages.dtype != vPages.dtype or kPages.transposed or vPages.transposed:
+        if len(kPages.shape) != 4 or min(kPages.shape[1:]) < 1 or kPages.shape != vPages.shape or kPages.dtype != vPages.dtype or kPages.transposed or vPages.transposed:
             raise TlError(B.TL_ERR_INVALID_ARG, "createPagedCache: kPages and vPages are [nPages, kvH, pageSize, D] of one dtype")
         if kPages.dtype not in B.DTYPE_ID:
             raise TlError(B.TL_ERR_INVALID_ARG, f"createPagedCache: pages of dtype {kPages.dtype}")
