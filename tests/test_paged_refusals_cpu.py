@@ -20,3 +20,15 @@ def test_a_cache_without_heads_slots_or_dimensions_is_refused(be, shape):  # noq
     with pytest.raises(tb.TlError, match="createPagedCache"):
         tb.PagedCache(be, _t(be, shape), _t(be, shape), _t(be, [3, 4], "i32"))
     tb.PagedCache(be, _t(be, [0, 2, 16, 64]), _t(be, [0, 2, 16, 64]), _t(be, [0, 0], "i32"))  # one without pages yet is not
+
+
+def test_a_window_past_32_bits_is_none_and_a_negative_one_is_refused(be):  # noqa: F811
+    cache, pos, q = _paged(be), _t(be, [3], "i32"), _t(be, [3, 4, 64])
+    for window, told in ((0, 0), (7, 7), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (2 ** 32, 2 ** 31 - 1), (2 ** 32 + 5, 2 ** 31 - 1)):
+        be.ops.pagedAttention(cache, pos, q, 0.1, window=window)
+        assert be.calls[-1][0] == "tl_paged_attention" and be.calls[-1][-2] == told
+    calls = len(be.calls)
+    for window in (-1, -2 ** 32, -2 ** 32 + 3):
+        with pytest.raises(tb.TlError, match="window"):
+            be.ops.pagedAttention(cache, pos, q, 0.1, window=window)
+    assert len(be.calls) == calls

@@ -429,12 +429,15 @@ class CudaOps:
             _refuse("pagedAttention: q is [tokens, H, D] of the cache's dtype")
         if slopes is not None and (slopes.dtype != "f32" or slopes.shape != [heads]):
             _refuse("pagedAttention: slopes are f32 [H]")
+        window = min(int(window), 2 ** 31 - 1)  # the library takes 32 bits, which no position leaves
+        if window < 0:
+            _refuse("pagedAttention: the window is negative")
         if out is None:
             out = self.empty([tokens, heads * d], cache.dtype)
         elif out.dtype != cache.dtype or out.transposed or (out.shape != [tokens, heads * d] and out.shape != [tokens, heads, d]):
             _refuse("pagedAttention: out is [tokens, H * D] of the cache's dtype")
         self._b._calls.tl_paged_attention(self._b._handle, cache.descriptor(), positions.buffer, tokenSeq.buffer if tokenSeq is not None else None,
-                                          tokens, q.buffer, heads * d, d, heads, out.buffer, float(scale), float(softcap), int(window),
+                                          tokens, q.buffer, heads * d, d, heads, out.buffer, float(scale), float(softcap), window,
                                           slopes.buffer if slopes is not None else None)
         return out
 

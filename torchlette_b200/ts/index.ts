@@ -294,9 +294,11 @@ export function pagedAttention(cache: PagedCache, positions: CudaTensor, q: Cuda
   const tokens = tokensOf("pagedAttention", positions, tokenSeq), heads = q.shape.length === 3 ? q.shape[1] : q.shape.length === 2 ? q.shape[1] / d : 0;
   refuseUnless(heads >= 1 && Number.isInteger(heads) && fits(q, dtype, [tokens, heads, d], [tokens, heads * d]), "pagedAttention: q is [tokens, H, D] of the cache's dtype");
   refuseUnless(fits(slopes, "f32", [heads]), "pagedAttention: slopes are f32 [H]");
+  const window = Math.min(config.window ?? 0, 2 ** 31 - 1); // the library takes 32 bits, which no position leaves
+  refuseUnless(window >= 0, "pagedAttention: the window is negative");
   refuseUnless(fits(config.out, dtype, [tokens, heads * d], [tokens, heads, d]), "pagedAttention: out is [tokens, H * D] of the cache's dtype");
   const out = config.out ?? empty([tokens, heads * d], dtype);
-  addon.pagedAttention(need(), p, positions.buffer, at(tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, scale, config.softcap ?? 0, config.window ?? 0, at(slopes));
+  addon.pagedAttention(need(), p, positions.buffer, at(tokenSeq), tokens, q.buffer, heads * d, d, heads, out.buffer, scale, config.softcap ?? 0, window, at(slopes));
   return out;
 }
 /** A token of each row of logits [rows, vocab] (any leading dims) from uniforms f32 [rows]; parameters f32 (topK: i32) [rows] or absent.  Returns i32 [rows], in `out`
