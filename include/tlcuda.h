@@ -369,7 +369,7 @@ TL_API int32_t tl_paged_append(tl_ctx* ctx, const tl_paged_cache* cache, const i
  *   x_j = q . k_j * scale;  softcap > 0: x_j = softcap * tanh(x_j / softcap);  slopes: x_j += slopes[h] * (j - p)  (f32 [n_heads])
  *   out = sum_j softmax(x)_j v_j, zeros where nothing is seen, NaN where a score that is seen is NaN or +infinity or all of them are -infinity.
  * Several tokens of one sequence in a call are rows of their own (each reads the cache).  head_dim is a multiple of 8, at most 256;
- * pages, q and out start on 16 bytes and the strides are multiples of 16 bytes.  softcap is 0 or at least 1e-30.  The context's calls share a
+ * pages, q and out start on 16 bytes and the strides are multiples of 16 bytes; out does not overlap q.  softcap is 0 or at least 1e-30.  The context's calls share a
  * scratch of fixed size, made by the first call (a call in a graph capture before it is refused): captured calls, too, are replayed one after another. */
 TL_API int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32_t* positions, const int32_t* token_seq, int64_t tokens,
                                   const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t n_heads, void* out, float scale,

@@ -1,8 +1,11 @@
 """More of what the backend refuses, or passes on as it is meant, in the paged cache's calls."""
+import ctypes as C
+
 import pytest
 
-from test_paged_cpu import _paged, _t, be  # noqa: F401
+from test_paged_cpu import ATTEND, AT, _cache, _paged, _t, be, ctx, stub  # noqa: F401
 from torchlette_b200 import backend as tb
+from torchlette_b200 import binding as B
 
 
 def test_transposed_tables_are_refused(be):  # noqa: F811
@@ -32,3 +35,10 @@ def test_a_window_past_32_bits_is_none_and_a_negative_one_is_refused(be):  # noq
         with pytest.raises(tb.TlError, match="window"):
             be.ops.pagedAttention(cache, pos, q, 0.1, window=window)
     assert len(be.calls) == calls
+
+
+def test_attention_over_its_own_queries_is_refused(ctx):  # noqa: F811
+    lib = B.load()
+    assert ATTEND["q"] == ATTEND["out"]
+    assert lib.tl_paged_attention(ctx, C.byref(_cache()), *ATTEND.values()) == B.TL_ERR_INVALID_ARG
+    assert b"overlaps" in lib.tl_last_error(ctx)

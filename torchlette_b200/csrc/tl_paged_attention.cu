@@ -1177,6 +1177,8 @@ int32_t tl_paged_attention(tl_ctx* ctx, const tl_paged_cache* cache, const int32
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache->k_pages) |
         reinterpret_cast<uintptr_t>(cache->v_pages)) & 15) != 0)
     return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_attention: pages, q, out and q's strides must be multiples of 16 bytes");
+  // A token's queries are read by more than one CTA, and again behind its first outputs where values are infinite
+  if (q == out) return tl_set_error(ctx, TL_ERR_INVALID_ARG, "tl_paged_attention: out overlaps q");
   DeviceGuard guard(ctx->device);
   rc = secure_scratch(ctx);
   if (rc != TL_OK) return rc;
