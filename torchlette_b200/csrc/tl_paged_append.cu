@@ -8,7 +8,7 @@
 //
 // Bound: HBM for prompts (every element is read and written once), launch and the chain position -> page -> store for a step's few tokens.  A head
 // is a group of lanes; a thread keeps its dimensions' rotation in registers and takes several heads of its token, whose loads are on their way together.
-// Measured: 8001 tokens x 48 heads x 128 bf16: 44.6 us (198 MB, 4.4 TB/s); a step's 64 tokens 4.5 us through the Python API, its host time.
+// Measured: 8001 tokens x 48 heads x 128 bf16: 40.8 us (198 MB, 4.85 TB/s), f32 65.2 (6.1 TB/s); a step's 64 tokens 4.6 us through the Python API, its host time.
 #include <algorithm>
 #include <type_traits>
 
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 1024 / THREADS : 768
 
 // A thread takes one head while the tokens are too few to fill the chip (their loads all at once), else as many of a token's as six, in smaller
 // CTAs: what a thread works out once (its token's place, pages and rotation) costs about as many instructions as two heads (8001 tokens x 48
-// heads x 128 bf16: 47 us with three heads a thread).
+// heads x 128 bf16: 47 us with three heads a thread, when six took 44.6).
 template <typename T, int LANES, int HEADS, int THREADS> cudaError_t launch_heads(tl_ctx* ctx, const AppendArgs& p, int rows) {
   constexpr int kRows = THREADS / LANES * HEADS;
   return tl_launch_waiting(append_vec_kernel<T, LANES, HEADS, THREADS>, dim3(unsigned(p.tokens), unsigned((rows + kRows - 1) / kRows)), dim3(THREADS), ctx->stream, p);

@@ -20,8 +20,8 @@
 // from accumulators to the B operand in the register file (movmatrix), split into 16-bit terms that keep nearly all bits (tl_attention.cuh).
 // f32: CUDA cores, a lane per D / 32 dimensions; the partial dot products of eight keys are summed over the lanes by exchanging halves.
 //
-// Measured: 8 sequences x 4000 keys, 32 query / 8 KV heads x 128 f16: 31.5 us (131 MB, 4.1 TB/s; about 4 us until the first tile, 20 of copies at 6, 7 of
-// meeting and joining); 64 ragged sequences up to 8000, bf16: 120 us (5.9 TB/s); one of 100 003 keys, 2 KV heads: 29.8 us.
+// Measured: 8 sequences x 4000 keys, 32 query / 8 KV heads x 128 f16: 31.4 us (131 MB, 4.2 TB/s; about 4 us until the first tile, 20 of copies at 6, 7 of
+// meeting and joining); 64 ragged sequences up to 8000, bf16: 119 us (5.9 TB/s); one of 100 003 keys, 2 KV heads: 29.8 us.
 //
 // Rows of a tile that the token does not see never count: their scores are replaced, not multiplied, and their values zeroed before the
 // product, whatever the pages hold there.

@@ -20,8 +20,8 @@
 // exp in 64 bits by a table of 2^(j/128) and a polynomial on what is left (Tang's table-driven method, 1989): ten operations where the library's exp takes
 // about three times as many.
 //
-// Measured: 64 rows x 151 936 f32, top-k 50 and top-p .95: 25.3 us (39 MB: 6 us of HBM, the rest is the cluster's meetings and the first CTA's ranking);
-// 16 such rows in f16, top-p .9 and min-p .02: 45 us, 8 of them the pass into bins (exponentials and shared atomics), 4 each the pass
+// Measured: 64 rows x 151 936 f32, top-k 50 and top-p .95: 25.2 us (39 MB: 6 us of HBM, the rest is the cluster's meetings and the first CTA's ranking);
+// 16 such rows in f16, top-p .9 and min-p .02: 44 us, 8 of them the pass into bins (exponentials and shared atomics), 4 each the pass
 // that sends a bin's tokens and the one over the kept masses, the rest meetings and reads of other CTAs' bins.
 #include <algorithm>
 #include <climits>
@@ -633,8 +633,8 @@ int32_t tl_sample(tl_ctx* ctx, const void* logits, int32_t dtype, int64_t rows, 
   p.vocab = int32_t(vocab);
   p.shift = 44;
   while (p.shift > 38 && (vocab >> (62 - p.shift)) != 0) --p.shift;  // the whole mass stays below 2^63
-  // CTAs of a row: as many as keep all rows in one wave of two CTAs an SM, each with a vector a thread; top-p over 151 936 logits with 16 against 8: 16 rows
-  // 45 and 53 us, one row 35 and 44
+  // CTAs of a row: as many as leave two places an SM for all rows' (a row's lie in one GPC, so that some rows may start late all the same), each with a vector a thread;
+  // top-p over 151 936 logits with 16 against 8: 16 rows 45 and 53 us, one row 35 and 44
   int ctas = 1;
   while (ctas < kMaxCluster && vocab > int64_t(ctas) * kThreads * 8 && rows * ctas * 2 <= 2 * int64_t(ctx->sm_count)) ctas *= 2;
   p.per_cta = int32_t(((vocab + ctas - 1) / ctas + 7) / 8 * 8);

@@ -1,4 +1,4 @@
-// Element access of the decode ops (tl_decode_ops.cu, tl_paged_append.cu, tl_paged_attention.cu): any storage type as f32, one element or eight
+// Element access of the decode ops (tl_decode_ops.cu, tl_paged_append.cu): any storage type as f32, one element or eight
 // at a time, and the sum over a warp.
 #pragma once
 
