@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from test_gpu_paged import Cache, assert_close, normal, run_attention, wrap
+from test_gpu_paged import OPTIONS, Cache, assert_close, attention_ref, normal, run_attention, wrap
 from test_gpu_paged_scores import reference
 from torchlette_b200 import binding as B
 
@@ -66,6 +66,31 @@ def test_values_behind_small_and_no_probabilities(backend, dtype):
     got = run_attention(backend, c, q, pos, None, 0.125)
     ref, slack = reference(c, q, lengths, 0.125)
     assert ref[:, 0, 4].isposinf().all() and ref[:, 0, 5].isnan().all()
+    compare(got, ref, slack, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("options", OPTIONS[1:], ids="+".join)
+def test_values_under_options(backend, dtype, page, options):
+    """Windows that see an infinity or no longer do, caps and biases, several tokens of a sequence."""
+    gen, options = torch.Generator(device="cuda").manual_seed(page), dict(options)
+    lengths = [400, 1200, 20]
+    c = Cache(backend, gen, lengths, 2, 128, page, dtype)
+    for i, n in enumerate(lengths):
+        c.fill(gen, i, n, dtype)
+        rows, slots = c.rows(i, n)
+        c.v[rows[n - 10], i % 2, slots[n - 10], 100] = INF
+        c.v[rows[n - 16], i % 2, slots[n - 16], 100] = -INF
+        c.v[rows[n // 2], 0, slots[n // 2], 31] = -INF
+    tokens = [(0, 399), (1, 1199), (2, 19), (0, 388), (0, 395), (1, 615), (1, -1), (2, 3), (1, 300)]
+    seq, pos = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in zip(*tokens))
+    q = normal(gen, (len(tokens), 12, 128), dtype)
+    if "slopes" in options:
+        options["slopes"] = torch.rand(12, generator=gen, device="cuda") / 20
+    got = run_attention(backend, c, q, pos, seq, 0.09, **options)
+    ref, slack = attention_ref(c, q, pos, seq.tolist(), 0.09, dtype=dtype, **options)
+    assert ref.isinf().any() or options == {"window": 1}
     compare(got, ref, slack, dtype)
 
 
